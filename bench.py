@@ -355,18 +355,17 @@ def main():
     n_streams = args.streams
     overlap = n_streams > 1
     torch.cuda.synchronize()
-    # The main stream carries the step's critical chain and is created with high priority (-1), the NMS stream with the
-    # default: measured 202.5 k against 201.0 k images/s (the dense gradient pass loses less to the NMS chain beside it).
+    # All streams have the default priority.
     if overlap:      # keep the legacy null stream (which the runtime orders against every other stream) out of the loop
-        torch.cuda.set_stream(torch.cuda.Stream(priority=int(os.environ.get("DH_BENCH_MAIN_PRIORITY", "-1"))))
+        torch.cuda.set_stream(torch.cuda.Stream())
     main_stream = torch.cuda.current_stream()
-    nms_stream = torch.cuda.Stream(priority=int(os.environ.get("DH_BENCH_NMS_PRIORITY", "0"))) if overlap else main_stream
+    nms_stream = torch.cuda.Stream() if overlap else main_stream
     loss_stream = torch.cuda.Stream() if n_streams == 3 else main_stream
     early = overlap and not args.autograd and args.early_positives
     nms_first = overlap and args.nms_first
     # diagnostic: how fast the main stream runs with no NMS chain beside it (the line is then marked invalid)
     skip_nms, skipped, first_call = bool(os.environ.get("DH_BENCH_SKIP_NMS")), {}, [True]
-    pos_stream = torch.cuda.Stream(priority=int(os.environ.get("DH_BENCH_POS_PRIORITY", "0"))) if early else None
+    pos_stream = torch.cuda.Stream() if early else None
     set_stream = torch.cuda.set_stream
     split = {"prev_stats": None, "reduced": None, "local_of_reduced": None}
 
@@ -656,7 +655,7 @@ def main():
             "loss_call": "crit(p,t) + torch.autograd.grad" if args.autograd else (
                 "crit.positives(p,t) on a side stream beside the decode, then crit.forward_backward(p,t,positives=...)" if early
                 else "crit.forward_backward(p,t)"),
-            "streams": {1: "one stream", 2: "decode, assign+loss (high-priority stream) | nms chain on two streams (stage_ms overlap)",
+            "streams": {1: "one stream", 2: "decode, assign+loss | nms chain on two streams (stage_ms overlap)",
                         3: "decode | nms chain | assign+loss on three streams (stage_ms overlap)"}[n_streams],
             "roofline": roofline,
         }

@@ -41,9 +41,9 @@ typedef float dh_f2 __attribute__((ext_vector_type(2)));
 // n / d of two pairs at once, correctly rounded for operands in the "plain" range (below).  The instruction sequence is the
 // one the compiler expands an IEEE fp32 division into -- reciprocal estimate, one refinement of it, two refinements of the
 // quotient -- without the three instructions around it that only matter outside that range (v_div_scale of numerator and
-// denominator, v_div_fixup), and on two pairs per instruction (v_pk_fma_f32): 4.5 vector instructions per quotient instead of
-// 10.  The kernel is bound by exactly those instructions at write-bound sizes (counters: 24 per element, the vector ALU busy
-// for 41 of 47 us at 8192 x 8192).
+// denominator, v_div_fixup): 7 vector instructions per quotient instead of 10.  The kernel is bound by exactly those
+// instructions at write-bound sizes (counters with the full division: 24 per element, the vector ALU busy for 41 of 47 us at
+// 8192 x 8192).
 __device__ __forceinline__ dh_f2 pw_div2_plain(const dh_f2 n, const dh_f2 d)
 {
     const dh_f2 one = {1.0f, 1.0f};

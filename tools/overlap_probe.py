@@ -17,8 +17,8 @@ strides = torch.tensor([8., 16., 32.])
 grads = [torch.empty_like(x) for x in levels]
 hyp = crit._hyp_struct()
 shapes = [(x.shape[2], x.shape[3]) for x in levels]
-main = torch.cuda.Stream(priority=-1)
-side = torch.cuda.Stream(priority=int(os.environ.get("SIDE_PRIO", "0")))
+main = torch.cuda.Stream()
+side = torch.cuda.Stream()
 lib = L.lib()
 
 
