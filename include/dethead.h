@@ -522,6 +522,44 @@ int dh_regression_loss_fwd(const float* pred, const float* target, const float* 
 int dh_regression_loss_bwd(const float* pred, const float* target, const float* mask, int64_t B, int64_t S, int smooth,
                            const float* out2, const float* grad_out, float* grad_pred, void* stream);
 
+/* ---- Matrix products with bias, activation and residual in the epilogue, and their gradients ----
+ * C_b(i,j) = sum_r A_b(i,r) B_b(j,r) for every batch b, with I, J and R the extents of i, j and r.  The 1x1 convolutions of
+ * Detect (object_detection/yolov5/models/yolo.py:52) are such products over channel-major maps, a linear layer is one over
+ * rows; the gradients of both are products again.
+ *   out(i,j) = act(C(i,j) + bias) + residual(i,j);  z (optional) receives C(i,j) + bias, which the backward of the
+ *   activation reads.  Sums are fp32; out and z are rounded once, to the type of the operands.
+ * A(i,r) is at a[b*a_batch + i*lda + r] when a_by_reduction, else at a[b*a_batch + r*lda + i]; B likewise.  out(i,j) is at
+ * out[b*o_batch + i*ldo + j], z at the same place, residual at residual[b*res_batch + i*ldr + j].  bias is indexed by i
+ * (bias_on_i) or by j.  reduce_batch: the batch is part of the reduction, out has no batch (a weight's gradient).
+ * Strides are in elements.  bias, residual and z may be null; out must not overlap the inputs, except that residual may be
+ * out itself.  All n products (at most DH_MAX_PRODUCTS) run in one launch (a second one where the reduction is split over
+ * workgroups) and share dtype, activation and the two *_by_reduction flags; the pair a_by_reduction = 0,
+ * b_by_reduction = 1 is not offered (exchange A and B).  Any alignment of the element type is accepted; 16-byte aligned
+ * pointers and strides are faster.  workspace: 16-byte aligned, dh_products_workspace() bytes (may be 0); the same products
+ * captured into two graphs that run at once need two of them. */
+#define DH_MAX_PRODUCTS 5
+enum { DH_F32 = 0, DH_F16 = 1, DH_BF16 = 2 };
+enum { DH_ACT_NONE = 0, DH_ACT_RELU = 1, DH_ACT_SILU = 2, DH_ACT_GELU = 3, DH_ACT_SIGMOID = 4, DH_ACT_LAST = 4 };
+typedef struct dh_product {
+    const void *a, *b, *bias, *residual;
+    void *out, *z;
+    int64_t lda, ldb, ldo, ldr;
+    int64_t a_batch, b_batch, o_batch, res_batch;
+    int I, J, R, batch;
+    int a_by_reduction, b_by_reduction, bias_on_i, reduce_batch;
+} dh_product;
+size_t dh_products_workspace(const dh_product* products, int n, int dtype);
+int dh_products(const dh_product* products, int n, int dtype, int activation, void* workspace, size_t workspace_bytes,
+                void* stream);
+
+/* The two other steps of those products' backward pass, in one read of dy: dz = dy * act'(z) (skipped when z is null) and the
+ * bias gradient dbias[c] = sum over outer and inner of dz (skipped when dbias is null; summed before dz is rounded).  dy, z
+ * and dz are contiguous [outer][n][inner]: maps have inner = cells, rows inner = 1.  workspace: device,
+ * dh_product_slope_workspace(n) bytes when dbias is given. */
+size_t dh_product_slope_workspace(int64_t n);
+int dh_product_slope(const void* dy, const void* z, void* dz, void* dbias, int64_t outer, int64_t n, int64_t inner,
+                     int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Measurement aid, no counterpart in the reference: copies `bytes` (a multiple of 16, both pointers 16-byte aligned) with
  * one 16-byte non-temporal load and store per thread.  bench.py times it on the bytes of one decode launch: the copy rate
  * this memory system gives a kernel that only moves data, reported beside the nominal 8 TB/s. */

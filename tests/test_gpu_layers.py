@@ -1,0 +1,391 @@
+"""Products with bias, activation and residual in the epilogue, and their gradients, against 64 bits (tests/_products.py)."""
+import ctypes
+
+import pytest
+import torch
+
+from tests._products import close, rows64, to_maps, to_rows
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+ACTS = [None, "relu", "silu", "gelu", "sigmoid"]
+
+
+def made(shape, dtype, seed, factor=1.0, whole=False):
+    """Seeded values; `whole`: small integers, whose products and sums are exact (a relu's border is then exactly zero)."""
+    g = torch.Generator().manual_seed(seed)
+    if whole:
+        return torch.randint(-3, 4, shape, generator=g).to(dtype)
+    return (torch.randn(shape, generator=g) * factor).to(dtype)
+
+
+def rows_case(m, k, n, dtype, act, bias, residual, seed=0):
+    whole = act == "relu"
+    x = made((m, k), dtype, seed, whole=whole)
+    w = made((n, k), dtype, seed + 1, max(k, 1) ** -0.5, whole=whole)
+    b = made((n,), dtype, seed + 2, 0.5, whole=whole) if bias else None
+    r = made((m, n), dtype, seed + 3) if residual else None
+    dy = made((m, n), dtype, seed + 4)
+    return x, w, b, r, dy
+
+
+def leaves(*tensors):
+    return [t.cuda().requires_grad_(True) if t is not None else None for t in tensors]
+
+
+def check_rows(m, k, n, dtype, act, bias, residual):
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = rows_case(m, k, n, dtype, act, bias, residual)
+    want = rows64(x, w, b, act, r, dy)
+    label = f"rows {m}x{k}->{n} {dtype} {act}"
+    with torch.no_grad():
+        y = linear(x.cuda(), w.cuda(), b.cuda() if bias else None, act, r.cuda() if residual else None)
+    assert y.shape == (m, n) and y.dtype == dtype
+    close(y, want["y"], label + " y")
+    gx, gw, gb, gr = leaves(x, w, b, r)
+    y2 = linear(gx, gw, gb, act, gr)
+    assert torch.equal(y2.detach(), y)                      # the same arithmetic with and without a backward to come
+    y2.backward(dy.cuda())
+    close(gx.grad, want["dx"], label + " dx")
+    close(gw.grad, want["dw"], label + " dw")
+    if bias:
+        close(gb.grad, want["db"], label + " db")
+    if residual:
+        assert torch.equal(gr.grad.cpu(), dy)
+
+
+SIZES = [(1, 1, 1), (1, 64, 64), (3, 5, 7), (2, 8, 264), (17, 129, 65), (64, 64, 64), (128, 64, 128), (130, 200, 257), (65, 1000, 33),
+         (7, 2049, 12), (200, 24, 8), (513, 72, 136)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+def test_rows_sizes(size, dtype):
+    check_rows(*size, dtype, "silu", True, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True), (True, True)])
+def test_rows_epilogues(act, dtype, bias, residual):
+    check_rows(37, 72, 88, dtype, act, bias, residual)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(4096, 256, 512), (1, 4096, 1024), (9, 4096, 777), (2000, 40, 40)])
+def test_rows_larger(size, dtype):
+    check_rows(*size, dtype, "gelu", True, False)
+
+
+MAPS = [(1, 1, 1, 1, 1), (2, 16, 255, 5, 7), (1, 130, 65, 13, 13), (3, 64, 64, 8, 8), (2, 33, 130, 20, 20), (5, 8, 24, 1, 3),
+        (1, 512, 255, 4, 4), (2, 128, 255, 40, 40), (70, 16, 16, 2, 2)]
+
+
+def check_maps(b, k, n, ny, nx, dtype, act, residual, layout=torch.contiguous_format):
+    from object_detection_amd.layers import pointwise_conv
+    whole = act == "relu"
+    x = made((b, k, ny, nx), dtype, 1, whole=whole).contiguous(memory_format=layout)
+    w = made((n, k, 1, 1), dtype, 2, k ** -0.5, whole=whole)
+    bias = made((n,), dtype, 3, 0.5, whole=whole)
+    r = made((b, n, ny, nx), dtype, 4) if residual else None
+    dy = made((b, n, ny, nx), dtype, 5)
+    want = rows64(to_rows(x), w.reshape(n, k), bias, act, to_rows(r) if residual else None, to_rows(dy))
+    label = f"maps {b}x{k}x{ny}x{nx}->{n} {dtype} {act} {layout}"
+    gx, gw, gb, gr = leaves(x, w, bias, r)
+    y = pointwise_conv(gx, gw, gb, act, gr)
+    assert y.shape == (b, n, ny, nx) and y.dtype == dtype
+    close(to_rows(y), want["y"], label + " y")
+    y.backward(dy.cuda())
+    close(to_rows(gx.grad), want["dx"], label + " dx")
+    close(gw.grad.reshape(n, k), want["dw"], label + " dw")
+    close(gb.grad, want["db"], label + " db")
+    if residual:
+        assert torch.equal(gr.grad.cpu(), dy)
+    return y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", MAPS)
+def test_maps_sizes(size, dtype):
+    check_maps(*size, dtype, "silu", True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ACTS)
+def test_maps_activations(act, dtype):
+    check_maps(2, 40, 48, 6, 6, dtype, act, False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_maps_channels_last(dtype):
+    y = check_maps(2, 40, 72, 5, 6, dtype, "silu", True, torch.channels_last)
+    assert y.is_contiguous(memory_format=torch.channels_last)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_head_levels(dtype):
+    """Three levels of different widths and sizes in one launch; one level without a bias."""
+    from object_detection_amd.layers import head_convs
+    geometry = [(16, 12, 12), (40, 6, 6), (129, 3, 3)]
+    xs = [made((3, c, h, w), dtype, 10 + c) for c, h, w in geometry]
+    ws = [made((75, c, 1, 1), dtype, 20 + c, c ** -0.5) for c, _, _ in geometry]
+    bs = [made((75,), dtype, 30), None, made((75,), dtype, 31)]
+    dys = [made((3, 75, h, w), dtype, 40 + h) for _, h, w in geometry]
+    gx, gw, gb = leaves(*xs), leaves(*ws), leaves(*bs)
+    ys = head_convs(gx, gw, gb)
+    torch.autograd.backward(ys, [d.cuda() for d in dys])
+    for l in range(3):
+        want = rows64(to_rows(xs[l]), ws[l].reshape(75, -1), bs[l], None, None, to_rows(dys[l]))
+        assert ys[l].shape == dys[l].shape
+        close(to_rows(ys[l]), want["y"], f"level {l} y")
+        close(to_rows(gx[l].grad), want["dx"], f"level {l} dx")
+        close(gw[l].grad.reshape(75, -1), want["dw"], f"level {l} dw")
+        if bs[l] is not None:
+            close(gb[l].grad, want["db"], f"level {l} db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset", [0, 1, 8])
+def test_rows_inside_a_wider_tensor(dtype, offset):
+    """x and the residual as column slices of tensors whose other columns are NaN: nothing around a row is read into it."""
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = rows_case(70, 40, 56, dtype, "silu", True, True)
+    wide = torch.full((70, 40 + offset + 9), float("nan"), dtype=dtype, device="cuda")
+    wide_r = torch.full((70, 56 + offset + 8), float("nan"), dtype=dtype, device="cuda")
+    wide[:, offset:offset + 40] = x.cuda()
+    wide_r[:, offset:offset + 56] = r.cuda()
+    gx, gr = wide[:, offset:offset + 40].detach().requires_grad_(True), wide_r[:, offset:offset + 56].detach().requires_grad_(True)
+    assert not gx.is_contiguous()
+    gw, gb = leaves(w, b)
+    y = linear(gx, gw, gb, "silu", gr)
+    want = rows64(x, w, b, "silu", r, dy)
+    close(y, want["y"], "y")
+    y.backward(dy.cuda())
+    close(gx.grad, want["dx"], "dx")
+    close(gw.grad, want["dw"], "dw")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_maps_inside_a_wider_tensor(dtype):
+    """Channels of a wider map (a concatenation's slice), its other channels NaN; odd cells, so nothing is aligned."""
+    from object_detection_amd.layers import pointwise_conv
+    x, w = made((3, 20, 5, 5), dtype, 1), made((17, 20), dtype, 2, 0.2)
+    wide = torch.full((3, 27, 5, 5), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 3:23] = x.cuda()
+    with torch.no_grad():
+        y = pointwise_conv(wide[:, 3:23], w.cuda())
+    close(to_rows(y), rows64(to_rows(x), w, None, None, None)["y"], "y")
+
+
+def test_broadcast_residual_and_gradient():
+    """An expanded residual and an expanded output gradient (sum()) are read and differentiated as what they stand for."""
+    from object_detection_amd.layers import linear
+    x, w, b, _, _ = rows_case(24, 16, 40, torch.float32, "silu", True, False)
+    row = made((1, 40), torch.float32, 9)
+    gx, gw, gb, grow = leaves(x, w, b, row)
+    linear(gx, gw, gb, "silu", grow.expand(24, 40)).sum().backward()
+    want = rows64(x, w, b, "silu", row.expand(24, 40), torch.ones(24, 40))
+    close(gx.grad, want["dx"], "dx")
+    close(gw.grad, want["dw"], "dw")
+    close(gb.grad, want["db"], "db")
+    assert torch.equal(grow.grad.cpu(), torch.full((1, 40), 24.0))
+
+
+def test_the_same_tensor_twice():
+    """x as its own residual (y = act(x W^T) + x): its gradient is the sum of both paths."""
+    from object_detection_amd.layers import linear
+    x, w, b, _, dy = rows_case(19, 48, 48, torch.float32, "silu", True, False)
+    gx, gw = leaves(x, w)
+    y = linear(gx, gw, b.cuda(), "silu", gx)
+    y.backward(dy.cuda())
+    want = rows64(x, w, b, "silu", x, dy)
+    close(y, want["y"], "y")
+    value, bound = want["dx"]
+    close(gx.grad, (value + dy.double(), bound + 2 * 2.0 ** -24 * (value.abs() + dy.abs())), "dx")
+
+
+@pytest.mark.parametrize("size", [(0, 8, 8), (5, 0, 9), (5, 8, 0), (0, 0, 3)])
+def test_empty(size):
+    from object_detection_amd.layers import linear
+    m, k, n = size
+    x, w, b, r, dy = rows_case(m, k, n, torch.float32, "silu", True, True)
+    want = rows64(x, w, b, "silu", r, dy)
+    gx, gw, gb, gr = leaves(x, w, b, r)
+    y = linear(gx, gw, gb, "silu", gr)
+    assert y.shape == (m, n)
+    close(y, want["y"], "y")
+    y.backward(dy.cuda())
+    for g, name in ((gx, "dx"), (gw, "dw"), (gb, "db")):
+        close(g.grad, want[name], name)
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    """An infinite or NaN input reaches its own output row only, as in the definition."""
+    from object_detection_amd.layers import linear
+    for dtype in DTYPES:
+        x, w, b, _, _ = rows_case(140, 72, 130, dtype, None, True, False)
+        want = rows64(x, w, b, None, None)["y"]
+        x[7, 3], x[20, 71], x[139, 0] = float("nan"), float("inf"), float("-inf")
+        with torch.no_grad():
+            y = linear(x.cuda(), w.cuda(), b.cuda()).cpu()
+        special = [7, 20, 139]
+        exact = x.double()[special] @ w.double().t() + b.double()
+        assert torch.equal(torch.isnan(y[special]), torch.isnan(exact))
+        finite = ~torch.isnan(exact)
+        assert torch.equal(y[special].double()[finite], exact[finite])
+        rest = torch.ones(140, dtype=torch.bool)
+        rest[special] = False
+        close(y[rest], (want[0][rest], want[1][rest]), f"rest {dtype}")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_activations_far_out(act):
+    """Pre-activations from -1e4 to 1e4: no overflow on the way, the limits of the functions at the ends."""
+    from object_detection_amd.layers import linear
+    z = torch.tensor([-1e4, -200.0, -100.0, -88.0, -20.0, -5.0, -1.0, -0.0, 0.0, 1.0, 5.0, 20.0, 88.0, 100.0, 200.0, 1e4])
+    x, w = z[:, None], torch.ones(1, 1)
+    want = rows64(x, w, None, act, None, torch.ones(16, 1))
+    gx = x.cuda().requires_grad_(True)
+    y = linear(gx, w.cuda(), activation=act)
+    y.sum().backward()
+    close(y, want["y"], "y")
+    close(gx.grad, want["dx"], "dx")
+
+
+def test_gradient_against_differences():
+    """The directional derivative of <dy, y> by central differences of the kernel itself (fp32): step h = 2^-6 has an error of
+    h^2/6 of the third derivative (|act'''| < 1.1 over the direction's projections, below 2e-4 of the terms' sum) and the
+    rounding of y, 2 (R + 4) u sum |dy| (|y| + 1) / h."""
+    from object_detection_amd.layers import linear
+    m, k, n, h = 12, 24, 20, 2.0 ** -6
+    for act in ("silu", "gelu", "sigmoid"):
+        x, w, b, r, dy = rows_case(m, k, n, torch.float32, act, True, True, seed=5)
+        vx, vw, vb = made((m, k), torch.float32, 50, 0.3), made((n, k), torch.float32, 51, 0.3 * k ** -0.5), made((n,), torch.float32, 52, 0.3)
+        t = [v.cuda() for v in (x, w, b, r, dy, vx, vw, vb)]
+
+        def value(s):
+            with torch.no_grad():
+                y = linear(t[0] + s * t[5], t[1] + s * t[6], t[2] + s * t[7], act, t[3])
+            return (y.double() * t[4].double()).sum()
+        gx, gw, gb = leaves(x, w, b)
+        linear(gx, gw, gb, act, t[3]).backward(t[4])
+        slope = sum((g.grad.double() * v.double()).sum() for g, v in ((gx, t[5]), (gw, t[6]), (gb, t[7])))
+        got = (value(h) - value(-h)) / (2 * h)
+        y = linear(*t[:3], act, t[3]).double()
+        # direction of z: (x + s vx)(w + s vw)^T is quadratic in s, its first and second derivatives bound the third of act(z(s))
+        z1 = (t[5] @ t[1].t() + t[0] @ t[6].t() + t[7]).double().abs()
+        z2 = 2 * (t[5] @ t[6].t()).double().abs()
+        third = 1.1 * z1 ** 3 + 3 * 0.8 * z1 * z2
+        bound = (t[4].double().abs() * (h * h / 6 * 1.5 * third + 2 * (k + 4) * 2.0 ** -24 * (y.abs() + 1) / h)).sum()
+        assert (got - slope).abs() < bound, (act, float(got), float(slope), float(bound))
+
+
+def test_autocast_casts_like_torch_layers():
+    from object_detection_amd.layers import head_convs, linear
+    x, w, b, _, _ = rows_case(9, 32, 24, torch.float32, None, True, False)
+    gx, gw, gb = leaves(x, w, b)
+    with torch.autocast("cuda", dtype=torch.float16):
+        y = linear(gx, gw, gb)
+        maps = head_convs([gx.view(1, 9, 32, 1).permute(0, 2, 1, 3)], [gw], [gb])[0]
+    assert y.dtype == torch.float16 and maps.dtype == torch.float16
+    y.float().sum().backward()
+    assert gx.grad.dtype == gw.grad.dtype == torch.float32
+    h = rows64(x.half(), w.half(), b.half(), None, None, torch.ones(9, 24, dtype=torch.float16))
+    close(y, h["y"], "y")
+    close(gx.grad, h["dx"], "dx")
+    close(maps.permute(0, 2, 3, 1).reshape(9, 24), h["y"], "maps")
+
+
+def test_same_bits_every_time():
+    """Split reductions are joined in a fixed order: outputs and gradients repeat bit for bit."""
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = rows_case(2000, 300, 40, torch.bfloat16, "silu", True, True)
+    runs = []
+    for _ in range(3):
+        gx, gw, gb = leaves(x, w, b)
+        y = linear(gx, gw, gb, "silu", r.cuda())
+        y.backward(dy.cuda())
+        runs.append([y.detach(), gx.grad, gw.grad, gb.grad])
+    for again in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(runs[0], again))
+
+
+def test_another_stream_and_graph_replay():
+    """The calls run on torch's current stream; captured into a graph (forward and gradients) they replay on new inputs."""
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = [t.cuda() for t in rows_case(50, 640, 72, torch.float16, "silu", True, True)]
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        eager = linear(x, w, b, "silu", r)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = linear(x, w, b, "silu", r)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(eager, other)
+    sx, sdy = x.clone().requires_grad_(True), dy.clone()
+    gw = w.clone().requires_grad_(True)
+
+    def step():
+        y = linear(sx, gw, b, "silu", r)
+        return (y.detach(),) + torch.autograd.grad(y, [sx, gw], sdy)
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            out = step()
+    torch.cuda.synchronize()
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (70, 71, 72):
+        fresh = made((50, 640), torch.float16, seed).cuda()
+        with torch.no_grad():
+            sx.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        want = step()
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)
+        del want
+
+
+def test_entry_leaves_everything_around_the_output():
+    """dh_products into the middle of a larger buffer: rows, columns and batches around the output keep their bits."""
+    from object_detection_amd import _lib as L
+    from object_detection_amd.layers import Product
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 2)):
+        for i, j, k, ldo in ((5, 7, 33, 12), (130, 129, 64, 136), (64, 64, 640, 64)):
+            a, b = made((i, k), dtype, 1).cuda(), made((j, k), dtype, 2).cuda()
+            frame = torch.full((i + 4, ldo), 77.0, dtype=dtype, device="cuda")
+            p = (Product * 1)(Product(a=a.data_ptr(), b=b.data_ptr(), out=frame[2].data_ptr(), lda=k, ldb=k, ldo=ldo, I=i, J=j, R=k,
+                                      batch=1, a_by_reduction=1, b_by_reduction=1))
+            need = L.lib().dh_products_workspace(p, 1, code)
+            ws = torch.full((need + 64,), 7, dtype=torch.uint8, device="cuda")
+            assert L.lib().dh_products(p, 1, code, 0, ctypes.c_void_p(ws.data_ptr()), need, L.stream()) == 0
+            torch.cuda.synchronize()
+            close(frame[2:2 + i, :j], rows64(a.cpu(), b.cpu(), None, None, None)["y"], f"{dtype} {i}x{j}")
+            keep = frame.clone()
+            keep[2:2 + i, :j] = 77.0
+            assert (keep == 77.0).all() and (ws[need:] == 7).all()
+
+
+def test_refuses_what_it_cannot_do():
+    from object_detection_amd.layers import head_convs, linear, pointwise_conv
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    for call in (lambda: linear(x, w.half()), lambda: linear(x.double(), w.double()), lambda: linear(x, w[:, :7]),
+                 lambda: linear(x, w, torch.zeros(5, device="cuda")), lambda: linear(x, w, residual=torch.zeros(4, 5, device="cuda")),
+                 lambda: linear(x, w.cpu()), lambda: linear(x, torch.zeros(6, 8, 1, 1, device="cuda")),
+                 lambda: pointwise_conv(x, w), lambda: pointwise_conv(x.view(1, 8, 2, 2), torch.zeros(6, 8, 3, 3, device="cuda")),
+                 lambda: pointwise_conv(x.view(1, 8, 2, 2), w, residual=torch.zeros(1, 6, 2, 3, device="cuda")),
+                 lambda: head_convs([], [], []), lambda: head_convs([x.view(1, 8, 2, 2)] * 6, [w] * 6, [None] * 6),
+                 lambda: head_convs([x.view(1, 8, 2, 2)], [w, w], [None]),
+                 lambda: head_convs([x.view(1, 8, 2, 2), x.half().view(1, 8, 2, 2)], [w, w.half()], [None, None])):
+        with pytest.raises(RuntimeError):
+            call()
+    with pytest.raises(ValueError):
+        linear(x, w, activation="softmax")
+    y = linear(x.requires_grad_(True), w, activation="silu")
+    g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
