@@ -560,6 +560,24 @@ size_t dh_product_slope_workspace(int64_t n);
 int dh_product_slope(const void* dy, const void* z, void* dz, void* dbias, int64_t outer, int64_t n, int64_t inner,
                      int activation, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Norm of many gradients as one vector, and clipping ----
+ * norm = (sum over all elements of |g / scale|^p)^(1/p) for p = 1, 2 or infinity; the clipped gradient is
+ * g / scale * min(1, max_norm / (norm + 1e-6)).  Lists are host arrays of device pointers (element-aligned, any length, also
+ * empty tensors); they are read before the call returns.  scale: one device float (a loss scale) or null for 1.
+ * dh_grad_power writes dh_grad_parts(n, count) doubles, the sums (p = infinity: maxima) of its workgroups; lists of different
+ * types write theirs one after the other into one array.  dh_grad_clip reads all `parts` of them, in their order, and scales
+ * its list: out[k] may be grads[k] (then a factor of 1 writes nothing), out_dtype is dtype or DH_F32; norm_out (optional)
+ * receives the norm.  dh_grad_norm only joins the parts: `sum` (optional, double) the sum of powers, which several processes
+ * can add up and hand to dh_grad_clip as one part; `out` (optional, float) the norm.  Infinite or NaN elements give an
+ * infinite or NaN norm, and then a factor of 0 or NaN. */
+enum { DH_NORM_MAX = 0, DH_NORM_1 = 1, DH_NORM_2 = 2 };
+int64_t dh_grad_parts(const int64_t* n, int count);
+int dh_grad_power(const void* const* grads, const int64_t* n, int count, int dtype, int norm, double* partial, int64_t parts,
+                  void* stream);
+int dh_grad_norm(const double* partial, int64_t parts, int norm, const float* scale, double* sum, float* out, void* stream);
+int dh_grad_clip(const void* const* grads, void* const* out, const int64_t* n, int count, int dtype, int out_dtype, int norm,
+                 const double* partial, int64_t parts, const float* scale, double max_norm, float* norm_out, void* stream);
+
 /* Measurement aid, no counterpart in the reference: copies `bytes` (a multiple of 16, both pointers 16-byte aligned) with
  * one 16-byte non-temporal load and store per thread.  bench.py times it on the bytes of one decode launch: the copy rate
  * this memory system gives a kernel that only moves data, reported beside the nominal 8 TB/s. */

@@ -122,6 +122,11 @@ SIGNATURES = {
     "dh_products": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "dh_product_slope_workspace": (c_size_t, [c_i64]),
     "dh_product_slope": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_i64, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "dh_grad_parts": (c_i64, [c_void_p, c_int]),
+    "dh_grad_power": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_i64, c_void_p]),
+    "dh_grad_norm": (c_int, [c_void_p, c_i64, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "dh_grad_clip": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_i64, c_void_p, c_double,
+                             c_void_p, c_void_p]),
     "dh_stream_copy": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
     "dh_box_iou": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_void_p]),
     "dh_wh_iou": (c_int, [c_void_p, c_void_p, c_void_p, c_i64, c_i64, c_void_p]),

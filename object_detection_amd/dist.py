@@ -54,6 +54,23 @@ def all_reduce_loss_sums(sums, group=None):
     return total
 
 
+def all_reduce_norm_power(power, norm_type, group=None):
+    """What the ranks' gradient shards add up to: the sum over the ranks of a one-element float64 tensor of summed powers
+    |g|^p, or its maximum for the infinity norm.  The input is left as it is; a host-side backend (gloo) takes it through the
+    host.  A NaN on one rank is a NaN on all of them."""
+    total = power.detach().clone()
+    if not (dist.is_available() and dist.is_initialized()):
+        return total
+    host = total.cpu() if total.is_cuda and dist.get_backend(group) == "gloo" else total
+    if norm_type == float("inf"):      # a maximum of the values, and of whether one is NaN (backends differ in how MAX treats NaN)
+        pair = torch.cat((torch.nan_to_num(host, nan=0.0, posinf=float("inf")), torch.isnan(host).to(host.dtype)))
+        dist.all_reduce(pair, op=dist.ReduceOp.MAX, group=group)
+        host = torch.where(pair[1:] > 0, torch.full_like(pair[:1], float("nan")), pair[:1])
+    else:
+        dist.all_reduce(host, op=dist.ReduceOp.SUM, group=group)
+    return host.to(total.device)
+
+
 def global_loss_stats(crit, group=None):
     """[lbox, lobj, lcls, n_pos] of the whole data-parallel batch from the last call of `crit` on every rank: one
     all-reduce of crit.last_sums, then the divisions (ComputeLoss.items_from_sums)."""

@@ -6,6 +6,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
+from .layers import head_convs
 
 
 _ANCHOR_CACHE = {}
@@ -347,13 +348,15 @@ class Detect(nn.Module):
     """Same constructor, buffers and forward contract as yolo.py:33-70.
 
     Training: returns the list of (bs,na,ny,nx,no) maps.  Eval: returns (decoded (bs,A,no), that list).
-    The 1x1 convolutions stay ordinary nn.Conv2d layers; what follows them (the layout change of yolo.py:54 and the
+    The 1x1 convolutions stay ordinary nn.Conv2d layers (one launch for all levels with fused_convs); what follows them (the layout change of yolo.py:54 and the
     decode arithmetic) is one launch in eval mode, and a layout-change launch with its own backward in training.
     """
     stride = None
     onnx_dynamic = False
     lazy_maps = False     # return the maps as permuted views of the convolution outputs (no copy of yolo.py:54);
     # ComputeLoss recognises them and works on the convolution outputs directly, gradients included
+    fused_convs = False   # run the 1x1 convolutions of all levels as one launch of the framework's own product (layers.head_convs),
+    # their gradients too; False: torch's convolutions, as before (the two differ in the order of their sums)
     half_arithmetic = True    # a half-precision head (model.half(), val.py:129-130) returns the fp16 decoded tensor of
     # yolo.py:56-70 with torch's fp16 roundings; False: fp16 maps are widened on load and decoded in fp32 to an fp32 tensor
     # (one launch instead of two, closer to the fp32 model's result, not what the reference computes)
@@ -383,7 +386,7 @@ class Detect(nn.Module):
             if half and self.half_arithmetic and not self.inplace:
                 return non_max_suppression(self([v for v in x])[0], conf_thres, iou_thres, classes, agnostic, multi_label, labels,
                                            max_det)
-            convs = [self.m[i](x[i]) for i in range(self.nl)]
+            convs = self._convolutions(x)
             return conv_nms(convs, self.na, self.anchors, self.stride, conf_thres, iou_thres, classes, agnostic, multi_label,
                             labels, max_det, half_arithmetic=half and self.half_arithmetic)
 
@@ -396,9 +399,15 @@ class Detect(nn.Module):
         anchor_grid = (self.anchors[i].clone() * self.stride[i]).view((1, self.na, 1, 1, 2)).expand((1, self.na, ny, nx, 2)).float()
         return grid, anchor_grid
 
+    def _convolutions(self, x):
+        """yolo.py:52 for every level."""
+        if self.fused_convs and all(type(m) is nn.Conv2d for m in self.m):
+            return head_convs(x[:self.nl], [m.weight for m in self.m], [m.bias for m in self.m])
+        return [self.m[i](x[i]) for i in range(self.nl)]
+
     def forward(self, x):
+        x[:self.nl] = self._convolutions(x)
         for i in range(self.nl):
-            x[i] = self.m[i](x[i])
             if not self.training and (self.onnx_dynamic or self.grid[i].shape[2:4] != x[i].shape[2:4]):   # yolo.py:57-58
                 self.grid[i], self.anchor_grid[i] = self._make_grid(int(x[i].shape[3]), int(x[i].shape[2]), i)
         if self.training and self.lazy_maps:
