@@ -12,6 +12,7 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_bf16.h>
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
@@ -40,27 +41,60 @@ template <> struct Elem<__bf16> {
     __device__ static __bf16 down(float v) { return (__bf16)v; }
 };
 
-__device__ __forceinline__ float act_value(float z, int act)
+// Activations and their derivatives.  FAST (results that are rounded to 16 bits): exp2 and the reciprocal from the hardware
+// (1 ulp each), and the error function by Abramowitz & Stegun 7.1.26, whose error of 1.5e-7 is far below a 16-bit step; a gelu
+// is 14 instructions instead of the library's 45, which at 8192 x 4096 outputs is 30 us of vector work.
+template <int ACT, bool FAST> struct Act;
+template <bool FAST> struct Act<DH_ACT_NONE, FAST> {
+    __device__ static float value(float z) { return z; }
+    __device__ static float slope(float) { return 1.f; }
+};
+template <bool FAST> struct Act<DH_ACT_RELU, FAST> {
+    __device__ static float value(float z) { return z > 0.f ? z : (z != z ? z : 0.f); }      // a NaN stays one
+    __device__ static float slope(float z) { return z > 0.f ? 1.f : 0.f; }
+};
+template <bool FAST> __device__ __forceinline__ float logistic(float z)
 {
-    switch (act) {
-    case DH_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);      // a NaN stays one
-    case DH_ACT_SILU: return z / (1.f + expf(-z));
-    case DH_ACT_SIGMOID: return 1.f / (1.f + expf(-z));
-    case DH_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    default: return z;
-    }
+    if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896f * z));
+    return 1.f / (1.f + expf(-z));
 }
-
-__device__ __forceinline__ float act_slope(float z, int act)
-{
-    switch (act) {
-    case DH_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case DH_ACT_SILU: { const float s = 1.f / (1.f + expf(-z)); return s * (1.f + z * (1.f - s)); }
-    case DH_ACT_SIGMOID: { const float s = 1.f / (1.f + expf(-z)); return s * (1.f - s); }
-    case DH_ACT_GELU:
-        return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-    default: return 1.f;
+template <bool FAST> struct Act<DH_ACT_SILU, FAST> {
+    __device__ static float value(float z) { return FAST ? z * logistic<true>(z) : z / (1.f + expf(-z)); }
+    __device__ static float slope(float z) { const float s = logistic<FAST>(z); return s * (1.f + z * (1.f - s)); }
+};
+template <bool FAST> struct Act<DH_ACT_SIGMOID, FAST> {
+    __device__ static float value(float z) { return logistic<FAST>(z); }
+    __device__ static float slope(float z) { const float s = logistic<FAST>(z); return s * (1.f - s); }
+};
+template <bool FAST> struct Act<DH_ACT_GELU, FAST> {
+    // the normal distribution function at z; bell: exp(-z^2 / 2)
+    __device__ static float normal(float z, float* bell)
+    {
+        if (!FAST) {
+            *bell = expf(-0.5f * z * z);
+            return 0.5f * (1.f + erff(z * 0.70710678118654752f));
+        }
+        const float x = fabsf(z) * 0.70710678118654752f;
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+        *bell = __builtin_amdgcn_exp2f(-0.72134752044448f * z * z);
+        float h = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        h = fmaf(h, t, 0.5f * 1.421413741f);
+        h = fmaf(h, t, 0.5f * -0.284496736f);
+        h = fmaf(h, t, 0.5f * 0.254829592f) * t * *bell;      // (1 - erf(x)) / 2
+        return z > 0.f ? 1.f - h : h;
     }
+    __device__ static float value(float z) { float bell; return z * normal(z, &bell); }
+    __device__ static float slope(float z) { float bell; const float n = normal(z, &bell); return fmaf(z * 0.39894228040143268f, bell, n); }
+};
+
+// f.template operator()<ACT>() for the activation of a launch
+template <typename F> __device__ __forceinline__ void with_act(int act, F&& f)
+{
+    if (act == DH_ACT_NONE) f(std::integral_constant<int, DH_ACT_NONE>());
+    else if (act == DH_ACT_RELU) f(std::integral_constant<int, DH_ACT_RELU>());
+    else if (act == DH_ACT_SILU) f(std::integral_constant<int, DH_ACT_SILU>());
+    else if (act == DH_ACT_GELU) f(std::integral_constant<int, DH_ACT_GELU>());
+    else f(std::integral_constant<int, DH_ACT_SIGMOID>());
 }
 
 struct Plan {               // one problem of a launch and how it is cut
@@ -70,8 +104,7 @@ struct Plan {               // one problem of a launch and how it is cut
     int batch_steps;        // reduction steps of one batch
     int split, per;         // workgroups along the reduction, and steps of each
     int out_batches;        // batches of the output (1 when the batch is reduced)
-    int first;              // first workgroup of this problem
-    int vec_out;            // rows of out / z / residual can be accessed in 16-byte pieces
+    int first, count;       // first workgroup of this problem (a multiple of 8), and how many it has
     float* partial;         // split > 1: [split][out_batches][I][J]
 };
 
@@ -79,27 +112,6 @@ struct Launch {
     Plan plan[DH_MAX_PRODUCTS];
     int n, total, act;
 };
-
-// 16 bytes of an operand that is contiguous along the direction of `at` (extent `end`); elements beyond it are zero.
-template <typename T, bool VEC>
-__device__ __forceinline__ u4 load_chunk(const T* __restrict__ row, int at, int end)
-{
-    constexpr int CH = Elem<T>::CH;
-    u4 v = {0, 0, 0, 0};
-    if (VEC) {                                  // aligned, and the extent is a multiple of the chunk
-        if (at < end) v = *reinterpret_cast<const u4*>(row + at);
-    } else if (at + CH <= end) {
-        __builtin_memcpy(&v, row + at, 16);     // any alignment of the element type
-    } else {
-        T e[CH];
-        __builtin_memset(e, 0, 16);
-#pragma unroll
-        for (int k = 0; k < CH; ++k)
-            if (at + k < end) e[k] = row[at + k];
-        __builtin_memcpy(&v, e, 16);
-    }
-    return v;
-}
 
 // An operand's tile in LDS.  X: rows of the tile along the operand's own index, BR: along the reduction.
 //   R (contiguous along the reduction): [X][BR], one row is 128 bytes = 8 chunks; chunk c of row x sits at c ^ key(x), so that
@@ -120,20 +132,6 @@ struct Tile {
         if (RC) return PAIR ? ((row & 3) | ((row >> 1) & 4)) : (row & 7);
         if (sizeof(T) == 4) return (((row >> 2) & 3) * 4) & (ROW_CHUNKS - 1);
         return ((row & 3) * (PAIR ? 4 : 2)) & (ROW_CHUNKS - 1);
-    }
-
-    // chunk number k of the tile in memory order
-    template <bool VEC>
-    __device__ static u4 fetch(const T* __restrict__ base, int64_t ld, int x0, int xend, int r0, int rend, int k)
-    {
-        const int row = k / ROW_CHUNKS, c = k % ROW_CHUNKS;
-        if (RC) {
-            const int x = x0 + row < xend ? x0 + row : xend - 1;      // rows behind the end repeat the last: never stored
-            return load_chunk<T, VEC>(base + (int64_t)x * ld, r0 + c * CH, rend);
-        }
-        u4 zero = {0, 0, 0, 0};
-        if (r0 + row >= rend) return zero;
-        return load_chunk<T, VEC>(base + (int64_t)(r0 + row) * ld, x0 + c * CH, xend);
     }
 
     __device__ static void store(T* lds, int k, u4 v)
@@ -193,167 +191,439 @@ template <> __device__ __forceinline__ f4 mma16<__bf16>(s8 a, s8 b, f4 c)
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
 
-// The last step on N consecutive values of a row of C: bias, activation, residual, rounding.
-template <typename T, int N>
-__device__ __forceinline__ void finish(const dh_product& p, int act, bool vec, int b, int i, int j, int J, const float* acc)
+// How an operand's tile comes from memory to LDS.
+//
+// Stream (everything aligned to 16 bytes): the copy goes from memory to LDS without passing through registers.  The hardware
+// puts lane l's 16 bytes at M0 + 16 l, so the swizzle is applied to the address that each lane reads.  Offsets are set once; a
+// reduction step only moves the scalar base.  The copies are written in assembly because the compiler, which cannot tell the
+// ring's buffers apart, would wait for all of them before every fragment read; the kernel waits with vmcnt itself.
+template <typename T, int X, int BR, bool RC, bool PAIR, int THREADS>
+struct Stream {
+    typedef Tile<T, X, BR, RC, PAIR> TL;
+    static constexpr int CH = Elem<T>::CH, N = TL::CHUNKS / THREADS, ROWS = THREADS / TL::ROW_CHUNKS;
+    static_assert(TL::CHUNKS % THREADS == 0 && THREADS % TL::ROW_CHUNKS == 0, "whole rows of chunks per pass");
+    uint32_t offset[N];         // bytes from the tile's origin
+    const char* base;           // the tile's origin at the current step
+    int64_t step;               // bytes
+
+    __device__ void begin(const T* operand, int64_t ld, int x0, int xend, int r0)
+    {
+        const int row = threadIdx.x / TL::ROW_CHUNKS, slot = threadIdx.x % TL::ROW_CHUNKS;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int y = row + k * ROWS, c = slot ^ TL::key(y);
+            // what lies behind the operand's end repeats its last row or column: those sums are not stored
+            const int64_t o = RC ? (int64_t)(x0 + y < xend ? y : xend - 1 - x0) * ld + c * CH
+                                 : (int64_t)y * ld + (x0 + c * CH < xend ? c * CH : xend - CH - x0);
+            offset[k] = (uint32_t)(o * (int64_t)sizeof(T));
+        }
+        base = (const char*)(operand + (RC ? (int64_t)x0 * ld + r0 : (int64_t)r0 * ld + x0));
+        step = (RC ? BR : BR * ld) * (int64_t)sizeof(T);
+    }
+
+    // copies the step's chunks to `lds` (the wave's own first slot) and moves on; `left`: reduction values that remain
+    __device__ void copy(T* lds, int left)
+    {
+        const uint32_t to = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) T*)lds);
+        if (left >= BR) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) one(to + k * THREADS * 16, offset[k]);
+        } else {                // the end of the reduction: zeros behind it
+            const int row = threadIdx.x / TL::ROW_CHUNKS, slot = threadIdx.x % TL::ROW_CHUNKS, lane = threadIdx.x & 63;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int y = row + k * ROWS, c = slot ^ TL::key(y);
+                if (RC ? c * CH < left : y < left) one(to + k * THREADS * 16, offset[k]);
+                else *reinterpret_cast<u4*>(lds + (k * THREADS + lane) * CH) = u4{0, 0, 0, 0};
+            }
+            asm volatile("s_waitcnt vmcnt(0)" : : : "memory");      // a wave may have skipped some: the count is not N
+        }
+        base += step;
+    }
+
+    __device__ void one(uint32_t to, uint32_t from) const
+    {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(from), "s"(base) : "memory");
+    }
+};
+
+// Waits until at most N of this wave's copies are on their way and its LDS reads are done, then for the other waves.
+template <int N> __device__ __forceinline__ void wait_and_meet()
 {
-    const int64_t o = (int64_t)b * p.o_batch + (int64_t)i * p.ldo + j;
-    const int64_t ro = (int64_t)b * p.res_batch + (int64_t)i * p.ldr + j;
-    const T* bias = (const T*)p.bias;
-    const T* res = (const T*)p.residual;
-    const int n = J - j < N ? J - j : N;
-    const bool whole = vec && n == N;
-    alignas(16) T zs[N], ys[N], rs[N];
-    if (res) {
-        if (whole) __builtin_memcpy(rs, __builtin_assume_aligned(res + ro, N * sizeof(T) < 16 ? N * sizeof(T) : 16), sizeof(rs));
-        else
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// Feed (any alignment): through registers, one step ahead.
+template <typename T, int X, int BR, bool RC, bool PAIR, int THREADS>
+struct Feed {
+    typedef Tile<T, X, BR, RC, PAIR> TL;
+    static constexpr int CH = Elem<T>::CH, N = TL::CHUNKS / THREADS, ROWS = THREADS / TL::ROW_CHUNKS;
+    static_assert(TL::CHUNKS % THREADS == 0 && THREADS % TL::ROW_CHUNKS == 0, "whole rows of chunks per thread");
+    const T* at[N];
+    const T* last;          // the last address from which a whole chunk can be read
+    int64_t step;
+    bool live;              // C: this thread's columns exist
+    bool inside;            // the whole tile exists
+
+    __device__ void begin(const T* base, int64_t ld, int x0, int xend, int r0, int rend)
+    {
+        const int row = threadIdx.x / TL::ROW_CHUNKS, c = threadIdx.x % TL::ROW_CHUNKS;
 #pragma unroll
-            for (int k = 0; k < N; ++k) rs[k] = k < n ? res[ro + k] : T(0);
+        for (int k = 0; k < N; ++k) {
+            if (RC) {
+                const int x = x0 + row + k * ROWS;
+                at[k] = base + (int64_t)(x < xend ? x : xend - 1) * ld + r0 + c * CH;      // rows behind the end: never stored
+            } else {
+                at[k] = base + (int64_t)(r0 + row + k * ROWS) * ld + x0 + c * CH;
+            }
+        }
+        live = RC || x0 + c * CH < xend;
+        inside = x0 + X <= xend;
+        step = RC ? BR : BR * ld;
+        last = base + (RC ? (int64_t)(xend - 1) * ld + rend : (int64_t)(rend - 1) * ld + xend) - CH;
     }
+
+    // the chunks of a step of which `left` reduction values remain (BR or more: all); what lies behind them becomes zero
+    __device__ void fetch(u4* v, int left)
+    {
+        if (inside && left >= BR) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-        float z = acc[k];
-        if (bias) z += p.bias_on_i ? Elem<T>::up(bias[i]) : (k < n ? Elem<T>::up(bias[j + k]) : 0.f);
-        zs[k] = Elem<T>::down(z);
-        float y = act_value(z, act);
-        if (res) y += Elem<T>::up(rs[k]);
-        ys[k] = Elem<T>::down(y);
+            for (int k = 0; k < N; ++k) __builtin_memcpy(&v[k], at[k], 16);
+        } else {
+            const int row = threadIdx.x / TL::ROW_CHUNKS, c = threadIdx.x % TL::ROW_CHUNKS;
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                v[k] = u4{0, 0, 0, 0};
+                const int have = RC ? left - c * CH : (live && row + k * ROWS < left ? CH : 0);    // elements of the chunk that count
+                if (have >= CH && at[k] <= last) {
+                    __builtin_memcpy(&v[k], at[k], 16);
+                } else if (have > 0) {
+                    T e[CH];
+                    __builtin_memset(e, 0, 16);
+#pragma unroll
+                    for (int q = 0; q < CH; ++q)
+                        if (q < have && at[k] + q < last + CH) e[q] = at[k][q];
+                    __builtin_memcpy(&v[k], e, 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < N; ++k) at[k] += step;
     }
-    T* out = (T*)p.out + o;
-    T* zout = p.z ? (T*)p.z + o : nullptr;
-    if (whole) {
-        __builtin_memcpy(__builtin_assume_aligned(out, N * sizeof(T) < 16 ? N * sizeof(T) : 16), ys, sizeof(ys));
-        if (zout) __builtin_memcpy(__builtin_assume_aligned(zout, N * sizeof(T) < 16 ? N * sizeof(T) : 16), zs, sizeof(zs));
+
+    __device__ static void stage(T* lds, const u4* v)
+    {
+#pragma unroll
+        for (int k = 0; k < N; ++k) TL::store(lds, k * THREADS + threadIdx.x, v[k]);
+    }
+};
+
+// One reduction step of a wave's tile from LDS.
+template <typename T, typename TA, typename TB, int BR, int TI, int TJ>
+__device__ __forceinline__ void multiply(f4 (&acc)[TI][TJ], const T* la, const T* lb, int wi, int wj, int lane)
+{
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int kk = 0; kk < BR / 16; ++kk) {
+            f4 fa[TI], fb[TJ];
+#pragma unroll
+            for (int b = 0; b < TJ; ++b) fb[b] = TB::frag32(lb, wj, b, kk, lane);
+#pragma unroll
+            for (int a = 0; a < TI; ++a) fa[a] = TA::frag32(la, wi, a, kk, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int a = 0; a < TI; ++a)
+#pragma unroll
+                    for (int b = 0; b < TJ; ++b)
+                        acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
+        }
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k)
-            if (k < n) { out[k] = ys[k]; if (zout) zout[k] = zs[k]; }
+        for (int kk = 0; kk < BR / 32; ++kk) {
+            s8 fa[TI], fb[TJ];
+#pragma unroll
+            for (int b = 0; b < TJ; ++b) fb[b] = TB::frag16(lb, wj, b, kk, lane);
+#pragma unroll
+            for (int a = 0; a < TI; ++a) fa[a] = TA::frag16(la, wi, a, kk, lane);
+#pragma unroll
+            for (int a = 0; a < TI; ++a)
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<T>(fb[b], fa[a], acc[a][b]);
+        }
     }
 }
 
-template <typename T, int BI, int BJ, int WI, int WJ, bool ARC, bool BRC, bool VEC>
-__global__ void __launch_bounds__(WI * WJ * 64) k_product(const Launch L)
+// Which tile of which product a workgroup has.  Consecutive workgroup numbers go to the 8 XCDs in turn: each XCD takes a
+// contiguous eighth of every product's tiles, in groups of 8 tiles along i that pass over j together, so that the tiles that run
+// at one time on an XCD share their operands in its L2.
+struct Place {
+    int w, i0, j0, batch, s;
+};
+__device__ __forceinline__ bool place(const Launch& L, int BI, int BJ, Place* at)
 {
-    constexpr bool F32 = sizeof(T) == 4;
-    constexpr int BR = F32 ? 32 : 64;
+    int w = 0;
+    while (w + 1 < L.n && (int)blockIdx.x >= L.plan[w + 1].first) ++w;
+    const Plan& q = L.plan[w];
+    const int local = (int)blockIdx.x - q.first, per = (q.count + 7) / 8;       // q.first is a multiple of 8
+    int tile = (local & 7) * per + (local >> 3);
+    if ((local >> 3) >= per || tile >= q.count) return false;
+    const int plane = q.tiles_i * q.tiles_j;
+    const int rest = tile / plane;
+    tile -= rest * plane;
+    const int group = tile / (8 * q.tiles_j), in = tile - group * 8 * q.tiles_j;
+    const int height = q.tiles_i - group * 8 < 8 ? q.tiles_i - group * 8 : 8;
+    const int tj = in / height;
+    at->w = w;
+    at->i0 = (group * 8 + in - tj * height) * BI;
+    at->j0 = tj * BJ;
+    at->s = rest / q.out_batches;
+    at->batch = rest - at->s * q.out_batches;
+    return true;
+}
+
+// What happens to a wave's accumulators.  They hold C in squares (a lane has four consecutive j of one row), memory wants rows:
+// 16 rows at a time go through LDS (`mine`: 16 x W floats that only this wave uses), after which a lane has 16 bytes of the
+// result's row and its neighbours the bytes beside them.  What is read from memory is requested before anything is stored.
+template <typename T, typename TB, int TI, int TJ>
+__device__ __forceinline__ void epilogue(f4 (&acc)[TI][TJ], const Plan& q, int act, const Place& at, int i0, int j0, float* mine)
+{
+    const dh_product& p = q.p;
+    const int I = p.I, J = p.J, ob = at.batch, lane = threadIdx.x & 63;
+    constexpr int V = Elem<T>::CH, W = TJ * 16, LANES = W / V, ROWS = 64 / LANES < 16 ? 64 / LANES : 16, PASSES = 16 / ROWS;
+    constexpr int MASK = W / 4 - 1 < 15 ? W / 4 - 1 : 15;
+    const int r = lane / LANES, jl = lane % LANES * V, j = j0 + jl;
+    const bool live = j < J && r < ROWS, whole = j + V <= J;
+    const bool joined = q.split > 1;                // partial sums: nothing but them, in fp32
+    const T* bias = joined ? nullptr : (const T*)p.bias;
+    const T* rp = joined ? nullptr : (const T*)p.residual;
+    T* zp = joined ? nullptr : (T*)p.z;
+    u4 res[TI][PASSES];
+    float bi[TI][PASSES], bj[V];
+    if (rp) {
+        rp += (int64_t)ob * p.res_batch + j;
+#pragma unroll
+        for (int a = 0; a < TI; ++a)
+#pragma unroll
+            for (int n = 0; n < PASSES; ++n) {
+                const int i = i0 + 16 * a + ROWS * n + r;
+                res[a][n] = u4{0, 0, 0, 0};
+                if (i < I && live) {
+                    const T* from = rp + (int64_t)i * p.ldr;
+                    if (whole) {
+                        __builtin_memcpy(&res[a][n], from, 16);
+                    } else {
+                        T t[V];
+                        __builtin_memset(t, 0, 16);
+#pragma unroll
+                        for (int e = 0; e < V - 1; ++e)
+                            if (j + e < J) t[e] = from[e];
+                        __builtin_memcpy(&res[a][n], t, 16);
+                    }
+                }
+            }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) bj[e] = 0.f;
+    if (bias && !p.bias_on_i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) bj[e] = Elem<T>::up(bias[j + e < J ? j + e : J - 1]);
+    }
+#pragma unroll
+    for (int a = 0; a < TI; ++a)
+#pragma unroll
+        for (int n = 0; n < PASSES; ++n) {
+            const int i = i0 + 16 * a + ROWS * n + r;
+            bi[a][n] = bias && p.bias_on_i ? Elem<T>::up(bias[i < I ? i : I - 1]) : 0.f;
+        }
+#pragma unroll
+    for (int a = 0; a < TI; ++a) {
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");        // the rows before have been read
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) {
+            const int m = lane & 15, c = TB::index(b, 4 * (lane >> 4)) / 4;
+            *reinterpret_cast<f4*>(mine + m * W + (c ^ (m & MASK)) * 4) = acc[a][b];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");        // the wave's lanes read what its other lanes wrote
+#pragma unroll
+        for (int n = 0; n < PASSES; ++n) {
+            const int row = ROWS * n + r, i = i0 + 16 * a + row;
+            if (!live || i >= I) continue;
+            float v[V];
+#pragma unroll
+            for (int h = 0; h < V / 4; ++h)
+                *reinterpret_cast<f4*>(v + 4 * h) = *reinterpret_cast<const f4*>(mine + row * W + ((jl / 4 + h) ^ (row & MASK)) * 4);
+            if (joined) {
+                float* o = q.partial + (((int64_t)at.s * q.out_batches + ob) * I + i) * J + j;
+                if (whole) __builtin_memcpy(o, v, 4 * V);
+                else
+#pragma unroll
+                    for (int e = 0; e < V - 1; ++e)
+                        if (j + e < J) o[e] = v[e];
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] += bi[a][n] + bj[e];          // (one of the two is zero)
+            auto store = [&](T* o) {
+                o += (int64_t)ob * p.o_batch + (int64_t)i * p.ldo + j;
+                alignas(16) T t[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) t[e] = Elem<T>::down(v[e]);
+                if (whole) __builtin_memcpy(o, t, 16);
+                else
+#pragma unroll
+                    for (int e = 0; e < V - 1; ++e)
+                        if (j + e < J) o[e] = t[e];
+            };
+            if (zp) store(zp);
+            with_act(act, [&](auto which) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = Act<decltype(which)::value, sizeof(T) == 2>::value(v[e]);
+            });
+            if (rp) {
+                T t[V];
+                __builtin_memcpy(t, &res[a][n], 16);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] += Elem<T>::up(t[e]);
+            }
+            store((T*)p.out);
+        }
+    }
+}
+
+// Aligned operands: a ring of STAGES buffers in LDS, the copies of STAGES - 1 steps on their way while one is multiplied.
+template <typename T, int BI, int BJ, int BR, int WI, int WJ, int STAGES, int WAVES, bool ARC, bool BRC>
+__global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
+{
     constexpr int THREADS = WI * WJ * 64;
     constexpr int TI = BI / WI / 16, TJ = BJ / WJ / 16;
-    constexpr bool PAIR = !F32;
-    typedef Tile<T, BI, BR, ARC, false> TA;
-    typedef Tile<T, BJ, BR, BRC, PAIR> TB;
-    constexpr int NA = TA::CHUNKS / THREADS, NB = TB::CHUNKS / THREADS;
-    static_assert(TA::CHUNKS % THREADS == 0 && TB::CHUNKS % THREADS == 0, "whole chunks per thread");
-    static_assert(!PAIR || TJ % 2 == 0, "fragments of B go in pairs");
-    __shared__ __align__(16) T lds_a[2][BI * BR];
-    __shared__ __align__(16) T lds_b[2][BJ * BR];
+    typedef Stream<T, BI, BR, ARC, false, THREADS> SA;
+    typedef Stream<T, BJ, BR, BRC, sizeof(T) == 2, THREADS> SB;
+    typedef typename SA::TL TA;
+    typedef typename SB::TL TB;
+    static_assert(sizeof(T) == 4 || TJ % 2 == 0, "fragments of B go in pairs");
+    __shared__ __align__(16) T lds[STAGES][(BI + BJ) * BR];
 
-    // consecutive workgroup numbers go to the 8 XCDs in turn: each XCD takes a contiguous eighth of the tiles, so that tiles
-    // which share an operand meet in one L2
-    const int per_xcd = (L.total + 7) / 8;
-    int tile = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (tile >= L.total) return;
-    int w = 0;
-    while (w + 1 < L.n && tile >= L.plan[w + 1].first) ++w;
-    const Plan& q = L.plan[w];
+    Place at;
+    if (!place(L, BI, BJ, &at)) return;
+    const Plan& q = L.plan[at.w];
     const dh_product& p = q.p;
-    tile -= q.first;
-    const int ti = tile % q.tiles_i; tile /= q.tiles_i;
-    const int tj = tile % q.tiles_j; tile /= q.tiles_j;
-    const int ob = tile % q.out_batches;
-    const int s = tile / q.out_batches;
-    const int i0 = ti * BI, j0 = tj * BJ;
-    const int k_begin = s * q.per, k_end = k_begin + q.per < q.steps ? k_begin + q.per : q.steps;
-
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int k_begin = at.s * q.per, k_end = k_begin + q.per < q.steps ? k_begin + q.per : q.steps;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
-    u4 ra[NA], rb[NB];
     f4 acc[TI][TJ];
 #pragma unroll
     for (int a = 0; a < TI; ++a)
 #pragma unroll
         for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
 
-    auto fetch = [&](int k) {
-        const int b = p.reduce_batch ? k / q.batch_steps : ob;
-        const int r0 = (p.reduce_batch ? k - b * q.batch_steps : k) * BR;
-        const T* A = (const T*)p.a + (int64_t)b * p.a_batch;
-        const T* B = (const T*)p.b + (int64_t)b * p.b_batch;
-#pragma unroll
-        for (int c = 0; c < NA; ++c) ra[c] = TA::template fetch<VEC>(A, p.lda, i0, p.I, r0, p.R, c * THREADS + tid);
-#pragma unroll
-        for (int c = 0; c < NB; ++c) rb[c] = TB::template fetch<VEC>(B, p.ldb, j0, p.J, r0, p.R, c * THREADS + tid);
+    SA sa;
+    SB sb;
+    int left = 0;                                    // reduction values of the current batch that are not requested yet
+    int batch = at.batch, asked = k_begin;
+    auto enter = [&](int r0) {
+        sa.begin((const T*)p.a + (int64_t)batch * p.a_batch, p.lda, at.i0, p.I, r0);
+        sb.begin((const T*)p.b + (int64_t)batch * p.b_batch, p.ldb, at.j0, p.J, r0);
+        left = p.R - r0;
     };
-    auto stage = [&](int at) {
-#pragma unroll
-        for (int c = 0; c < NA; ++c) TA::store(lds_a[at], c * THREADS + tid, ra[c]);
-#pragma unroll
-        for (int c = 0; c < NB; ++c) TB::store(lds_b[at], c * THREADS + tid, rb[c]);
+    if (k_begin < k_end) {
+        int r = k_begin;
+        if (p.reduce_batch) {
+            batch = k_begin / q.batch_steps;
+            r -= batch * q.batch_steps;
+        }
+        enter(r * BR);
+    }
+    auto ask = [&]() {
+        if (left <= 0) {                             // only a reduced batch has a next one
+            ++batch;
+            enter(0);
+        }
+        T* to = lds[(asked - k_begin) % STAGES] + wave * 64 * Elem<T>::CH;
+        sa.copy(to, left);
+        sb.copy(to + BI * BR, left);
+        left -= BR;
+        ++asked;
     };
-
-    if (k_begin < k_end) { fetch(k_begin); stage(0); }
-    __syncthreads();
-    int at = 0;
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k)
+        if (asked < k_end) ask();
     for (int k = k_begin; k < k_end; ++k) {
-        if (k + 1 < k_end) fetch(k + 1);
-        if constexpr (F32) {
-#pragma unroll
-            for (int kk = 0; kk < BR / 16; ++kk) {
-                f4 fa[TI], fb[TJ];
-#pragma unroll
-                for (int a = 0; a < TI; ++a) fa[a] = TA::frag32(lds_a[at], wi, a, kk, lane);
-#pragma unroll
-                for (int b = 0; b < TJ; ++b) fb[b] = TB::frag32(lds_b[at], wj, b, kk, lane);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int a = 0; a < TI; ++a)
-#pragma unroll
-                        for (int b = 0; b < TJ; ++b)
-                            acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
-            }
-        } else {
-#pragma unroll
-            for (int kk = 0; kk < BR / 32; ++kk) {
-                s8 fa[TI], fb[TJ];
-#pragma unroll
-                for (int a = 0; a < TI; ++a) fa[a] = TA::frag16(lds_a[at], wi, a, kk, lane);
-#pragma unroll
-                for (int b = 0; b < TJ; ++b) fb[b] = TB::frag16(lds_b[at], wj, b, kk, lane);
-#pragma unroll
-                for (int a = 0; a < TI; ++a)
-#pragma unroll
-                    for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<T>(fb[b], fa[a], acc[a][b]);
-            }
-        }
-        if (k + 1 < k_end) stage(at ^ 1);
-        __syncthreads();
-        at ^= 1;
+        if (asked - k == STAGES - 1) wait_and_meet<(STAGES - 2) * (SA::N + SB::N)>();
+        else wait_and_meet<0>();
+        if (asked < k_end) ask();
+        const T* from = lds[(k - k_begin) % STAGES];
+        multiply<T, TA, TB, BR, TI, TJ>(acc, from, from + BI * BR, wi, wj, lane);
     }
+    static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
+    __syncthreads();
+    epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
+}
 
-    // C's row i is the lane's column of the accumulator, its four values are consecutive in j (twice that for a pair)
-    constexpr int G = PAIR ? 2 : 1;
+// Any alignment: one buffer in LDS behind one step in registers.
+template <typename T, int BI, int BJ, int BR, int WI, int WJ, bool ARC, bool BRC>
+__global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
+{
+    constexpr int THREADS = WI * WJ * 64;
+    constexpr int TI = BI / WI / 16, TJ = BJ / WJ / 16;
+    typedef Feed<T, BI, BR, ARC, false, THREADS> FA;
+    typedef Feed<T, BJ, BR, BRC, sizeof(T) == 2, THREADS> FB;
+    typedef typename FA::TL TA;
+    typedef typename FB::TL TB;
+    __shared__ __align__(16) T lds[(BI + BJ) * BR];
+    T *lds_a = lds, *lds_b = lds + BI * BR;
+
+    Place at;
+    if (!place(L, BI, BJ, &at)) return;
+    const Plan& q = L.plan[at.w];
+    const dh_product& p = q.p;
+    const int k_begin = at.s * q.per, k_end = k_begin + q.per < q.steps ? k_begin + q.per : q.steps;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    FA feed_a;
+    FB feed_b;
+    u4 ra[FA::N], rb[FB::N];
+    f4 acc[TI][TJ];
 #pragma unroll
-    for (int a = 0; a < TI; ++a) {
-        const int i = i0 + wi + 16 * a + (lane & 15);
+    for (int a = 0; a < TI; ++a)
 #pragma unroll
-        for (int b = 0; b < TJ; b += G) {
-            const int j = j0 + wj + TB::index(b, 4 * (lane >> 4));
-            if (i >= p.I || j >= p.J) continue;
-            float v[4 * G];
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * g + e] = acc[a][b + g][e];
-            if (q.split > 1) {
-                float* o = q.partial + (((int64_t)s * q.out_batches + ob) * p.I + i) * p.J + j;
-#pragma unroll
-                for (int e = 0; e < 4 * G; ++e)
-                    if (j + e < p.J) o[e] = v[e];
-            } else {
-                finish<T, 4 * G>(p, L.act, q.vec_out != 0, ob, i, j, p.J, v);
-            }
+        for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
+
+    int left = 0, batch = at.batch;
+    auto enter = [&](int r0) {
+        feed_a.begin((const T*)p.a + (int64_t)batch * p.a_batch, p.lda, at.i0, p.I, r0, p.R);
+        feed_b.begin((const T*)p.b + (int64_t)batch * p.b_batch, p.ldb, at.j0, p.J, r0, p.R);
+        left = p.R - r0;
+    };
+    if (k_begin < k_end) {
+        int r = k_begin;
+        if (p.reduce_batch) {
+            batch = k_begin / q.batch_steps;
+            r -= batch * q.batch_steps;
         }
+        enter(r * BR);
     }
+    auto fetch = [&]() {
+        if (left <= 0) {
+            ++batch;
+            enter(0);
+        }
+        feed_a.fetch(ra, left);
+        feed_b.fetch(rb, left);
+        left -= BR;
+    };
+    if (k_begin < k_end) fetch();
+    for (int k = k_begin; k < k_end; ++k) {
+        __syncthreads();
+        FA::stage(lds_a, ra);
+        FB::stage(lds_b, rb);
+        __syncthreads();
+        if (k + 1 < k_end) fetch();
+        multiply<T, TA, TB, BR, TI, TJ>(acc, lds_a, lds_b, wi, wj, lane);
+    }
+    static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
+    __syncthreads();
+    epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
 // Sums the partial products of the workgroups along the reduction, in their order, and finishes them.
@@ -365,39 +635,59 @@ __global__ void __launch_bounds__(256) k_product_join(const Plan q, int act)
     for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
         float v = 0.f;
         for (int s = 0; s < q.split; ++s) v += q.partial[(int64_t)s * n + k];
-        const int j = (int)(k % p.J);
         const int64_t rest = k / p.J;
-        finish<T, 1>(p, act, false, (int)(rest / p.I), (int)(rest % p.I), j, p.J, &v);
+        const int j = (int)(k - rest * p.J), b = (int)(rest / p.I), i = (int)(rest - (int64_t)b * p.I);
+        if (p.bias) v += Elem<T>::up(((const T*)p.bias)[p.bias_on_i ? i : j]);
+        const int64_t o = (int64_t)b * p.o_batch + (int64_t)i * p.ldo + j;
+        if (p.z) ((T*)p.z)[o] = Elem<T>::down(v);
+        with_act(act, [&](auto a) { v = Act<decltype(a)::value, sizeof(T) == 2>::value(v); });
+        if (p.residual) v += Elem<T>::up(((const T*)p.residual)[(int64_t)b * p.res_batch + (int64_t)i * p.ldr + j]);
+        ((T*)p.out)[o] = Elem<T>::down(v);
     }
 }
 
-constexpr int TILE = 128, SMALL = 64;
+constexpr int CUS = 256;
+struct Shape { int bi, bj; };
 
-int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws_bytes, bool* vec, int* tile)
+// Tile shapes.  Large outputs: 128 x 128; where that leaves CUs without a tile: 64 x 64.
+Shape shape_of(const dh_product* ps, int n)
 {
-    const int64_t ch = dtype == DH_F32 ? 4 : 8, br = dtype == DH_F32 ? 32 : 64;
-    const int cus = 256;
     int64_t large = 0;
     for (int w = 0; w < n; ++w)
-        large += (int64_t)((ps[w].I + TILE - 1) / TILE) * ((ps[w].J + TILE - 1) / TILE) * (ps[w].reduce_batch ? 1 : ps[w].batch);
-    const int t = large >= cus ? TILE : SMALL;
-    *tile = t;
-    *vec = true;
+        large += (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * (ps[w].reduce_batch ? 1 : ps[w].batch);
+#ifdef DH_SWEEP
+    if (const char* e = getenv("DH_SHAPE")) { Shape s; sscanf(e, "%d,%d", &s.bi, &s.bj); return s; }
+#endif
+    return large >= CUS ? Shape{128, 128} : Shape{64, 64};
+}
+
+int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws_bytes, bool* aligned, Shape* shape)
+{
+    const int64_t ch = dtype == DH_F32 ? 4 : 8, br = dtype == DH_F32 ? 32 : 64, size = dtype == DH_F32 ? 4 : 2;
+    const Shape t = shape_of(ps, n);
+    *shape = t;
+    *aligned = true;
     int64_t total = 0;
     size_t bytes = 0;
+    int order[DH_MAX_PRODUCTS];
+    for (int w = 0; w < n; ++w) {          // long reductions first: their workgroups are the ones a launch waits for
+        int k = w;
+        for (; k > 0 && ps[order[k - 1]].R < ps[w].R; --k) order[k] = order[k - 1];
+        order[k] = w;
+    }
     for (int w = 0; w < n; ++w) {
-        const dh_product& p = ps[w];
+        const dh_product& p = ps[order[w]];
         Plan& q = L->plan[w];
         q.p = p;
-        q.tiles_i = (p.I + t - 1) / t;
-        q.tiles_j = (p.J + t - 1) / t;
+        q.tiles_i = (p.I + t.bi - 1) / t.bi;
+        q.tiles_j = (p.J + t.bj - 1) / t.bj;
         q.batch_steps = (int)((p.R + br - 1) / br);
         const int64_t steps = (int64_t)q.batch_steps * (p.reduce_batch ? p.batch : 1);
         q.out_batches = p.reduce_batch ? 1 : p.batch;
         const int64_t tiles = (int64_t)q.tiles_i * q.tiles_j * q.out_batches;
-        if (steps >= (1ll << 31) || tiles >= (1ll << 28)) return DH_ERR_ARG;
+        if (steps >= (1ll << 31) || tiles >= (1ll << 28) || (int64_t)q.tiles_i * q.tiles_j >= (1ll << 27)) return DH_ERR_ARG;
         q.steps = (int)steps;
-        int64_t split = tiles >= 2 * cus || tiles == 0 ? 1 : (2 * cus + tiles - 1) / tiles;
+        int64_t split = tiles >= 2 * CUS || tiles == 0 ? 1 : (2 * CUS + tiles - 1) / tiles;
         if (split > steps / 4) split = steps / 4;           // at least four steps each
         if (split < 1) split = 1;
         q.per = (int)((steps + split - 1) / split);
@@ -408,13 +698,13 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
             bytes += ((size_t)q.split * q.out_batches * p.I * p.J * sizeof(float) + 255) & ~(size_t)255;
         }
         q.first = (int)total;
-        total += tiles * q.split;
+        q.count = (int)(tiles * q.split);
+        total += (tiles * q.split + 7) / 8 * 8;
         if (total >= (1ll << 30)) return DH_ERR_ARG;
         const int64_t all = p.lda | p.ldb | p.a_batch | p.b_batch;
         const int64_t ea = p.a_by_reduction ? p.R : p.I, eb = p.b_by_reduction ? p.R : p.J;
-        if (all % ch || ea % ch || eb % ch || !dh_aligned16(p.a) || !dh_aligned16(p.b)) *vec = false;
-        q.vec_out = p.ldo % ch == 0 && p.o_batch % ch == 0 && dh_aligned16(p.out) && (!p.z || dh_aligned16(p.z)) &&
-                    (!p.residual || (p.ldr % ch == 0 && p.res_batch % ch == 0 && dh_aligned16(p.residual)));
+        if (all % ch || ea % ch || eb % ch || !dh_aligned16(p.a) || !dh_aligned16(p.b)) *aligned = false;
+        if ((p.lda > p.ldb ? p.lda : p.ldb) >= (1ll << 31) / (256 * size)) *aligned = false;       // offsets in a tile are 32 bits
     }
     L->n = n;
     L->total = (int)total;
@@ -422,27 +712,37 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     return DH_OK;
 }
 
-template <typename T, int B, bool ARC, bool BRC>
-void launch_tile(const Launch& L, bool vec, hipStream_t st)
+#ifdef DH_SWEEP
+#define DH_SHAPES(X) X(128, 128, 2, 2, 2, 2) X(64, 64, 2, 2, 2, 4) SWEEP_SHAPES(X)
+#else
+#define DH_SHAPES(X) X(128, 128, 2, 2, 2, 2) X(64, 64, 2, 2, 2, 4)
+#endif
+
+template <typename T, bool ARC, bool BRC>
+void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
 {
-    const dim3 grid((unsigned)((L.total + 7) / 8 * 8));
-    if (vec) hipLaunchKernelGGL((k_product<T, B, B, 2, 2, ARC, BRC, true>), grid, dim3(256), 0, st, L);
-    else hipLaunchKernelGGL((k_product<T, B, B, 2, 2, ARC, BRC, false>), grid, dim3(256), 0, st, L);
+    constexpr int BR = sizeof(T) == 4 ? 32 : 64;
+    const dim3 grid((unsigned)L.total);
+    if (aligned) {
+#define DH_CASE(BI, BJ, WI, WJ, STAGES, WAVES) \
+        if (t.bi == BI && t.bj == BJ) { \
+            hipLaunchKernelGGL((k_product<T, BI, BJ, BR, WI, WJ, STAGES, WAVES, ARC, BRC>), grid, dim3(WI * WJ * 64), 0, st, L); \
+            return; \
+        }
+        DH_SHAPES(DH_CASE)
+#undef DH_CASE
+    }
+    if (t.bi == 128) hipLaunchKernelGGL((k_product_any<T, 128, 128, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
+    else hipLaunchKernelGGL((k_product_any<T, 64, 64, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
 }
 
 template <typename T>
-int launch(const Launch& L, bool arc, bool brc, bool vec, int tile, hipStream_t st)
+int launch(const Launch& L, bool arc, bool brc, bool aligned, const Shape& t, hipStream_t st)
 {
     if (L.total > 0) {
-        if (tile == TILE) {
-            if (arc && brc) launch_tile<T, TILE, true, true>(L, vec, st);
-            else if (arc) launch_tile<T, TILE, true, false>(L, vec, st);
-            else launch_tile<T, TILE, false, false>(L, vec, st);
-        } else {
-            if (arc && brc) launch_tile<T, SMALL, true, true>(L, vec, st);
-            else if (arc) launch_tile<T, SMALL, true, false>(L, vec, st);
-            else launch_tile<T, SMALL, false, false>(L, vec, st);
-        }
+        if (arc && brc) launch_tiles<T, true, true>(L, aligned, t, st);
+        else if (arc) launch_tiles<T, true, false>(L, aligned, t, st);
+        else launch_tiles<T, false, false>(L, aligned, t, st);
     }
     for (int w = 0; w < L.n; ++w)
         if (L.plan[w].split > 1) {
@@ -477,6 +777,13 @@ int check(const dh_product* ps, int n, int dtype, int activation)
 // column block (inner == 1); their sums go to the workspace and are added in order by k_bias_join.
 constexpr int BIAS_SPLIT = 64;
 
+template <typename T> __device__ __forceinline__ float slope_of(float z, int act)
+{
+    float v = 1.f;
+    with_act(act, [&](auto a) { v = Act<decltype(a)::value, sizeof(T) == 2>::slope(z); });
+    return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) k_slope_planes(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
                                                       float* __restrict__ partial, int64_t outer, int64_t n, int64_t inner, int act)
@@ -487,7 +794,7 @@ __global__ void __launch_bounds__(256) k_slope_planes(const T* __restrict__ dy, 
         const int64_t at = (o * n + c) * inner;
         for (int64_t k = threadIdx.x; k < inner; k += 256) {
             float g = Elem<T>::up(dy[at + k]);
-            if (z) { g *= act_slope(Elem<T>::up(z[at + k]), act); dz[at + k] = Elem<T>::down(g); }
+            if (z) { g *= slope_of<T>(Elem<T>::up(z[at + k]), act); dz[at + k] = Elem<T>::down(g); }
             sum += g;
         }
     }
@@ -508,7 +815,7 @@ __global__ void __launch_bounds__(256) k_slope_rows(const T* __restrict__ dy, co
     if (c < n)
         for (int64_t r = s * 4 + (threadIdx.x >> 6); r < rows; r += 4 * BIAS_SPLIT) {
             float g = Elem<T>::up(dy[r * n + c]);
-            if (z) { g *= act_slope(Elem<T>::up(z[r * n + c]), act); dz[r * n + c] = Elem<T>::down(g); }
+            if (z) { g *= slope_of<T>(Elem<T>::up(z[r * n + c]), act); dz[r * n + c] = Elem<T>::down(g); }
             sum += g;
         }
     if (!partial) return;
@@ -552,9 +859,9 @@ extern "C" size_t dh_products_workspace(const dh_product* products, int n, int d
     if (check(products, n, dtype, 0) != DH_OK) return 0;
     Launch L;
     size_t bytes = 0;
-    bool vec;
-    int tile;
-    return cut(products, n, dtype, &L, nullptr, &bytes, &vec, &tile) == DH_OK ? bytes : 0;
+    bool aligned;
+    Shape shape;
+    return cut(products, n, dtype, &L, nullptr, &bytes, &aligned, &shape) == DH_OK ? bytes : 0;
 }
 
 extern "C" int dh_products(const dh_product* products, int n, int dtype, int activation, void* workspace, size_t workspace_bytes,
@@ -564,18 +871,18 @@ extern "C" int dh_products(const dh_product* products, int n, int dtype, int act
     if (rc != DH_OK) return rc;
     Launch L;
     size_t bytes = 0;
-    bool vec;
-    int tile;
-    rc = cut(products, n, dtype, &L, (float*)workspace, &bytes, &vec, &tile);
+    bool aligned;
+    Shape shape;
+    rc = cut(products, n, dtype, &L, (float*)workspace, &bytes, &aligned, &shape);
     if (rc != DH_OK) return rc;
     if (bytes > workspace_bytes || (bytes && !workspace)) return DH_ERR_WORKSPACE;
     if (bytes && !dh_aligned16(workspace)) return DH_ERR_ALIGN;
     L.act = activation;
     const bool arc = products[0].a_by_reduction != 0, brc = products[0].b_by_reduction != 0;
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == DH_F32) return launch<float>(L, arc, brc, vec, tile, st);
-    if (dtype == DH_F16) return launch<_Float16>(L, arc, brc, vec, tile, st);
-    return launch<__bf16>(L, arc, brc, vec, tile, st);
+    if (dtype == DH_F32) return launch<float>(L, arc, brc, aligned, shape, st);
+    if (dtype == DH_F16) return launch<_Float16>(L, arc, brc, aligned, shape, st);
+    return launch<__bf16>(L, arc, brc, aligned, shape, st);
 }
 
 extern "C" size_t dh_product_slope_workspace(int64_t n) { return n > 0 ? (size_t)n * BIAS_SPLIT * sizeof(float) : 0; }
