@@ -105,6 +105,7 @@ struct Plan {               // one problem of a launch and how it is cut
     int split, per;         // workgroups along the reduction, and steps of each
     int out_batches;        // batches of the output (1 when the batch is reduced)
     int first, count;       // first workgroup of this problem (a multiple of 8), and how many it has
+    int stream;             // out and z are stored past the caches, in 16-byte pieces
     float* partial;         // split > 1: [split][out_batches][I][J]
 };
 
@@ -129,6 +130,7 @@ struct Tile {
 
     __device__ static int key(int row)
     {
+        if (RC && ROW_CHUNKS == 4) return PAIR ? (((row >> 1) & 1) | ((row >> 2) & 2)) : ((row >> 1) & 3);
         if (RC) return PAIR ? ((row & 3) | ((row >> 1) & 4)) : (row & 7);
         if (sizeof(T) == 4) return (((row >> 2) & 3) * 4) & (ROW_CHUNKS - 1);
         return ((row & 3) * (PAIR ? 4 : 2)) & (ROW_CHUNKS - 1);
@@ -469,11 +471,17 @@ __device__ __forceinline__ void epilogue(f4 (&acc)[TI][TJ], const Plan& q, int a
                 alignas(16) T t[V];
 #pragma unroll
                 for (int e = 0; e < V; ++e) t[e] = Elem<T>::down(v[e]);
-                if (whole) __builtin_memcpy(o, t, 16);
-                else
+                if (whole && q.stream) {
+                    u4 w;
+                    __builtin_memcpy(&w, t, 16);
+                    __builtin_nontemporal_store(w, reinterpret_cast<u4*>(o));
+                } else if (whole) {
+                    __builtin_memcpy(o, t, 16);
+                } else {
 #pragma unroll
                     for (int e = 0; e < V - 1; ++e)
                         if (j + e < J) o[e] = t[e];
+                }
             };
             if (zp) store(zp);
             with_act(act, [&](auto which) {
@@ -647,26 +655,55 @@ __global__ void __launch_bounds__(256) k_product_join(const Plan q, int act)
 }
 
 constexpr int CUS = 256;
-struct Shape { int bi, bj; };
+struct Shape { int bi, bj, br, stages; };        // br: bytes of a reduction step's row
 
-// Tile shapes.  Large outputs: 128 x 128; where that leaves CUs without a tile: 64 x 64.
-Shape shape_of(const dh_product* ps, int n)
+// Tiles (i, j), bytes of a reduction step, waves along i and j, stages of the ring, waves per SIMD
+#define DH_SHAPES(X) X(128, 128, 128, 2, 2, 2, 2) X(128, 128, 64, 2, 2, 3, 3) X(64, 64, 128, 2, 2, 2, 4)
+#define DH_SHAPES_16(X) X(256, 256, 128, 2, 4, 2, 2)
+
+// The tile of a launch, by what it measured (us, bf16):
+//   256 x 256 (one workgroup of 8 waves per CU) where two of them per CU exist, they are at least 7/8 full and the reduction is
+//     long enough to pay for filling them: 8192 x 1024 -> 4096 72 against 83, 512 -> 256 channels of 64 x 80 x 80 cells 181 against
+//     210; but 128 -> 256 channels 95 against 76.
+//   128 x 128 in steps of 128 bytes and 2 stages where the reduction is long: 8192 x 4096 -> 1024 66 against 78; in steps of 64
+//     bytes and 3 stages (48 KB: three workgroups per CU) where it is short and loading, multiplying and storing have to
+//     overlap between workgroups: the head's levels (128 to 512 channels) at batch 64 119 against 159.
+//   64 x 64 where 128 x 128 would leave CUs without a tile.
+Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
 {
-    int64_t large = 0;
-    for (int w = 0; w < n; ++w)
-        large += (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * (ps[w].reduce_batch ? 1 : ps[w].batch);
-#ifdef DH_SWEEP
-    if (const char* e = getenv("DH_SHAPE")) { Shape s; sscanf(e, "%d,%d", &s.bi, &s.bj); return s; }
-#endif
-    return large >= CUS ? Shape{128, 128} : Shape{64, 64};
+    int64_t huge = 0, large = 0, held = 0;
+    int longest = 0;
+    for (int w = 0; w < n; ++w) {
+        const int64_t b = ps[w].reduce_batch ? 1 : ps[w].batch;
+        huge += (int64_t)((ps[w].I + 255) / 256) * ((ps[w].J + 255) / 256) * b;
+        large += (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * b;
+        held += (int64_t)ps[w].I * ps[w].J * b;
+        if (ps[w].R > longest) longest = ps[w].R;
+    }
+    if (large < CUS) return Shape{64, 64, 128, 2};
+    if (!aligned) return Shape{128, 128, 128, 1};
+    if (dtype != DH_F32 && huge >= 2 * CUS && longest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
+    return longest >= 1024 ? Shape{128, 128, 128, 2} : Shape{128, 128, 64, 3};
 }
 
 int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws_bytes, bool* aligned, Shape* shape)
 {
-    const int64_t ch = dtype == DH_F32 ? 4 : 8, br = dtype == DH_F32 ? 32 : 64, size = dtype == DH_F32 ? 4 : 2;
-    const Shape t = shape_of(ps, n);
-    *shape = t;
+    const int64_t ch = dtype == DH_F32 ? 4 : 8, size = dtype == DH_F32 ? 4 : 2;
     *aligned = true;
+    for (int w = 0; w < n; ++w) {
+        const dh_product& p = ps[w];
+        const int64_t all = p.lda | p.ldb | p.a_batch | p.b_batch;
+        const int64_t ea = p.a_by_reduction ? p.R : p.I, eb = p.b_by_reduction ? p.R : p.J;
+        if (all % ch || ea % ch || eb % ch || !dh_aligned16(p.a) || !dh_aligned16(p.b)) *aligned = false;
+        if ((p.lda > p.ldb ? p.lda : p.ldb) >= (1ll << 31) / (256 * size)) *aligned = false;       // offsets in a tile are 32 bits
+    }
+    const Shape t = shape_of(ps, n, dtype, *aligned);
+    const int64_t br = t.br / size;
+    *shape = t;
+    // Results that no cache could hold for their reader (32 MB of L2 in all) are stored past them.
+    int64_t written = 0;
+    for (int w = 0; w < n; ++w) written += (int64_t)ps[w].I * ps[w].J * (ps[w].reduce_batch ? 1 : ps[w].batch) * size * (ps[w].z ? 2 : 1);
+    const bool large = written > (32ll << 20);
     int64_t total = 0;
     size_t bytes = 0;
     int order[DH_MAX_PRODUCTS];
@@ -692,6 +729,7 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         if (split < 1) split = 1;
         q.per = (int)((steps + split - 1) / split);
         q.split = q.per ? (int)((steps + q.per - 1) / q.per) : 1;
+        q.stream = large && p.ldo % ch == 0 && p.o_batch % ch == 0 && dh_aligned16(p.out) && dh_aligned16(p.z);
         q.partial = nullptr;
         if (q.split > 1) {
             q.partial = (float*)((char*)ws + bytes);
@@ -701,10 +739,6 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         q.count = (int)(tiles * q.split);
         total += (tiles * q.split + 7) / 8 * 8;
         if (total >= (1ll << 30)) return DH_ERR_ARG;
-        const int64_t all = p.lda | p.ldb | p.a_batch | p.b_batch;
-        const int64_t ea = p.a_by_reduction ? p.R : p.I, eb = p.b_by_reduction ? p.R : p.J;
-        if (all % ch || ea % ch || eb % ch || !dh_aligned16(p.a) || !dh_aligned16(p.b)) *aligned = false;
-        if ((p.lda > p.ldb ? p.lda : p.ldb) >= (1ll << 31) / (256 * size)) *aligned = false;       // offsets in a tile are 32 bits
     }
     L->n = n;
     L->total = (int)total;
@@ -712,25 +746,24 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     return DH_OK;
 }
 
-#ifdef DH_SWEEP
-#define DH_SHAPES(X) X(128, 128, 2, 2, 2, 2) X(64, 64, 2, 2, 2, 4) SWEEP_SHAPES(X)
-#else
-#define DH_SHAPES(X) X(128, 128, 2, 2, 2, 2) X(64, 64, 2, 2, 2, 4)
-#endif
-
 template <typename T, bool ARC, bool BRC>
 void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
 {
-    constexpr int BR = sizeof(T) == 4 ? 32 : 64;
+    constexpr int BR = 128 / sizeof(T);
     const dim3 grid((unsigned)L.total);
     if (aligned) {
-#define DH_CASE(BI, BJ, WI, WJ, STAGES, WAVES) \
-        if (t.bi == BI && t.bj == BJ) { \
-            hipLaunchKernelGGL((k_product<T, BI, BJ, BR, WI, WJ, STAGES, WAVES, ARC, BRC>), grid, dim3(WI * WJ * 64), 0, st, L); \
+#define DH_CASE(BI, BJ, BYTES, WI, WJ, STAGES, WAVES) \
+        if (t.bi == BI && t.bj == BJ && t.br == BYTES && t.stages == STAGES) { \
+            hipLaunchKernelGGL((k_product<T, BI, BJ, BYTES / (int)sizeof(T), WI, WJ, STAGES, WAVES, ARC, BRC>), grid, dim3(WI * WJ * 64), 0, \
+                               st, L); \
             return; \
         }
         DH_SHAPES(DH_CASE)
+        if constexpr (sizeof(T) == 2) {
+            DH_SHAPES_16(DH_CASE)
+        }
 #undef DH_CASE
+        return;
     }
     if (t.bi == 128) hipLaunchKernelGGL((k_product_any<T, 128, 128, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
     else hipLaunchKernelGGL((k_product_any<T, 64, 64, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
