@@ -634,6 +634,106 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
+// One value of C through the epilogue.
+template <typename T> __device__ __forceinline__ void finish_one(const dh_product& p, int act, int b, int i, int j, float v)
+{
+    if (p.bias) v += Elem<T>::up(((const T*)p.bias)[p.bias_on_i ? i : j]);
+    const int64_t o = (int64_t)b * p.o_batch + (int64_t)i * p.ldo + j;
+    if (p.z) ((T*)p.z)[o] = Elem<T>::down(v);
+    with_act(act, [&](auto a) { v = Act<decltype(a)::value, sizeof(T) == 2>::value(v); });
+    if (p.residual) v += Elem<T>::up(((const T*)p.residual)[(int64_t)b * p.res_batch + (int64_t)i * p.ldr + j]);
+    ((T*)p.out)[o] = Elem<T>::down(v);
+}
+
+// Few rows of A (tokens) against many of B (a weight): bound by reading B once.  A workgroup of 8 waves takes 16 rows of B; its
+// waves take the reduction in turns of 128 bytes, fragments come from memory straight into registers (no row is used twice, so
+// LDS would only add a trip), and the waves' sums are added in order at the end.  Lane (m, g) reads 32 consecutive bytes of row
+// m, for two products of which each pairs the same reduction values of A and B; which values those are does not matter.
+template <typename T, int MI>
+__global__ void __launch_bounds__(512) k_product_thin(const Launch L)
+{
+    constexpr int CH = Elem<T>::CH, TURN = 8 * CH, WAVES = 8, AHEAD = 4 / MI;
+    __shared__ float sums[WAVES][MI * 256];
+    const Plan& q = L.plan[0];
+    const dh_product& p = q.p;
+    const int tile = (int)blockIdx.x % q.tiles_j, ob = (int)blockIdx.x / q.tiles_j;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, R = p.R, j0 = tile * 16;
+    const T* b = (const T*)p.b + (int64_t)ob * p.b_batch + (int64_t)(j0 + m < p.J ? j0 + m : p.J - 1) * p.ldb;
+    const T* a[MI];
+#pragma unroll
+    for (int n = 0; n < MI; ++n)
+        a[n] = (const T*)p.a + (int64_t)ob * p.a_batch + (int64_t)(16 * n + m < p.I ? 16 * n + m : p.I - 1) * p.lda;
+    f4 acc[MI];
+#pragma unroll
+    for (int n = 0; n < MI; ++n) acc[n] = f4{0.f, 0.f, 0.f, 0.f};
+
+    auto multiply = [&](const u4 (&vb)[2], const u4 (&va)[MI][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < MI; ++n) {
+                if constexpr (sizeof(T) == 4) {
+                    const f4 fb = __builtin_bit_cast(f4, vb[h]), fa = __builtin_bit_cast(f4, va[n][h]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[e], fa[e], acc[n], 0, 0, 0);
+                } else {
+                    acc[n] = mma16<T>(__builtin_bit_cast(s8, vb[h]), __builtin_bit_cast(s8, va[n][h]), acc[n]);
+                }
+            }
+    };
+    // the 2 CH values at k of a row; with an end: zeros from there on
+    auto whole = [&](const T* row, int k, u4 (&v)[2]) {
+        __builtin_memcpy(&v[0], row + k, 16);
+        __builtin_memcpy(&v[1], row + k + CH, 16);
+    };
+    auto some = [&](const T* row, int k, int end, u4 (&v)[2]) {
+        T e[2 * CH];
+#pragma unroll
+        for (int x = 0; x < 2 * CH; ++x) e[x] = k + x < end ? row[k + x] : T(0);
+        __builtin_memcpy(&v[0], e, 16);
+        __builtin_memcpy(&v[1], e + CH, 16);
+    };
+    const int turns = R / TURN;
+    int t = wave;
+    for (; t + (AHEAD - 1) * WAVES < turns; t += AHEAD * WAVES) {
+        u4 vb[AHEAD][2], va[AHEAD][MI][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int k = (t + u * WAVES) * TURN + g * 2 * CH;
+            whole(b, k, vb[u]);
+#pragma unroll
+            for (int n = 0; n < MI; ++n) whole(a[n], k, va[u][n]);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) multiply(vb[u], va[u]);
+    }
+    for (; t < turns; t += WAVES) {
+        u4 vb[2], va[MI][2];
+        const int k = t * TURN + g * 2 * CH;
+        whole(b, k, vb);
+#pragma unroll
+        for (int n = 0; n < MI; ++n) whole(a[n], k, va[n]);
+        multiply(vb, va);
+    }
+    if (t == turns && turns * TURN < R) {        // the wave whose turn it is takes what remains
+        u4 vb[2], va[MI][2];
+        const int k = t * TURN + g * 2 * CH;
+        some(b, k, R, vb);
+#pragma unroll
+        for (int n = 0; n < MI; ++n) some(a[n], k, R, va[n]);
+        multiply(vb, va);
+    }
+#pragma unroll
+    for (int n = 0; n < MI; ++n) *reinterpret_cast<f4*>(&sums[wave][n * 256 + m * 16 + 4 * g]) = acc[n];
+    __syncthreads();
+    const int i = threadIdx.x / 16, j = j0 + threadIdx.x % 16;
+    if (threadIdx.x >= MI * 256 || i >= p.I || j >= p.J) return;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v += sums[w][threadIdx.x];
+    finish_one<T>(p, L.act, ob, i, j, v);
+}
+
 // Sums the partial products of the workgroups along the reduction, in their order, and finishes them.
 template <typename T>
 __global__ void __launch_bounds__(256) k_product_join(const Plan q, int act)
@@ -645,17 +745,12 @@ __global__ void __launch_bounds__(256) k_product_join(const Plan q, int act)
         for (int s = 0; s < q.split; ++s) v += q.partial[(int64_t)s * n + k];
         const int64_t rest = k / p.J;
         const int j = (int)(k - rest * p.J), b = (int)(rest / p.I), i = (int)(rest - (int64_t)b * p.I);
-        if (p.bias) v += Elem<T>::up(((const T*)p.bias)[p.bias_on_i ? i : j]);
-        const int64_t o = (int64_t)b * p.o_batch + (int64_t)i * p.ldo + j;
-        if (p.z) ((T*)p.z)[o] = Elem<T>::down(v);
-        with_act(act, [&](auto a) { v = Act<decltype(a)::value, sizeof(T) == 2>::value(v); });
-        if (p.residual) v += Elem<T>::up(((const T*)p.residual)[(int64_t)b * p.res_batch + (int64_t)i * p.ldr + j]);
-        ((T*)p.out)[o] = Elem<T>::down(v);
+        finish_one<T>(p, act, b, i, j, v);
     }
 }
 
 constexpr int CUS = 256;
-struct Shape { int bi, bj, br, stages; };        // br: bytes of a reduction step's row
+struct Shape { int bi, bj, br, stages; };        // br: bytes of a reduction step's row; bi = 0: the thin kernel
 
 // Tiles (i, j), bytes of a reduction step, waves along i and j, stages of the ring, waves per SIMD
 #define DH_SHAPES(X) X(128, 128, 128, 2, 2, 2, 2) X(128, 128, 64, 2, 2, 3, 3) X(64, 64, 128, 2, 2, 2, 4)
@@ -680,6 +775,10 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
         held += (int64_t)ps[w].I * ps[w].J * b;
         if (ps[w].R > longest) longest = ps[w].R;
     }
+    // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs
+    const dh_product& p = ps[0];
+    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
+        return Shape{0, 16, 128, 1};
     if (large < CUS) return Shape{64, 64, 128, 2};
     if (!aligned) return Shape{128, 128, 128, 1};
     if (dtype != DH_F32 && huge >= 2 * CUS && longest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
@@ -716,7 +815,7 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         const dh_product& p = ps[order[w]];
         Plan& q = L->plan[w];
         q.p = p;
-        q.tiles_i = (p.I + t.bi - 1) / t.bi;
+        q.tiles_i = t.bi ? (p.I + t.bi - 1) / t.bi : p.I > 0;
         q.tiles_j = (p.J + t.bj - 1) / t.bj;
         q.batch_steps = (int)((p.R + br - 1) / br);
         const int64_t steps = (int64_t)q.batch_steps * (p.reduce_batch ? p.batch : 1);
@@ -724,7 +823,7 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         const int64_t tiles = (int64_t)q.tiles_i * q.tiles_j * q.out_batches;
         if (steps >= (1ll << 31) || tiles >= (1ll << 28) || (int64_t)q.tiles_i * q.tiles_j >= (1ll << 27)) return DH_ERR_ARG;
         q.steps = (int)steps;
-        int64_t split = tiles >= 2 * CUS || tiles == 0 ? 1 : (2 * CUS + tiles - 1) / tiles;
+        int64_t split = tiles >= 2 * CUS || tiles == 0 || t.bi == 0 ? 1 : (2 * CUS + tiles - 1) / tiles;
         if (split > steps / 4) split = steps / 4;           // at least four steps each
         if (split < 1) split = 1;
         q.per = (int)((steps + split - 1) / split);
@@ -751,6 +850,14 @@ void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
 {
     constexpr int BR = 128 / sizeof(T);
     const dim3 grid((unsigned)L.total);
+    if (t.bi == 0) {
+        if constexpr (ARC && BRC) {
+            const dim3 all((unsigned)L.plan[0].count);
+            if (L.plan[0].p.I <= 16) hipLaunchKernelGGL((k_product_thin<T, 1>), all, dim3(512), 0, st, L);
+            else hipLaunchKernelGGL((k_product_thin<T, 2>), all, dim3(512), 0, st, L);
+        }
+        return;
+    }
     if (aligned) {
 #define DH_CASE(BI, BJ, BYTES, WI, WJ, STAGES, WAVES) \
         if (t.bi == BI && t.bj == BJ && t.br == BYTES && t.stages == STAGES) { \
