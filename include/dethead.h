@@ -530,8 +530,10 @@ int dh_regression_loss_bwd(const float* pred, const float* target, const float* 
  *   activation reads.  Sums are fp32; out and z are rounded once, to the type of the operands.
  * A(i,r) is at a[b*a_batch + i*lda + r] when a_by_reduction, else at a[b*a_batch + r*lda + i]; B likewise.  out(i,j) is at
  * out[b*o_batch + i*ldo + j], z at the same place, residual at residual[b*res_batch + i*ldr + j].  bias is indexed by i
- * (bias_on_i) or by j.  reduce_batch: the batch is part of the reduction, out has no batch (a weight's gradient).
- * Strides are in elements.  bias, residual and z may be null; out must not overlap the inputs, except that residual may be
+ * (bias_on_i) or by j.  reduce_batch: the batch is part of the reduction, out has no batch (a weight's gradient).  a_sum
+ * (optional, I values of the type) receives the sums of A(i,r) over the reduction, batches included with reduce_batch: the
+ * bias gradient beside the weight's; only with reduce_batch or one batch.
+ * Strides are in elements.  bias, residual, z and a_sum may be null; out must not overlap the inputs, except that residual may be
  * out itself.  All n products (at most DH_MAX_PRODUCTS) run in one launch (a second one where the reduction is split over
  * workgroups) and share dtype, activation and the two *_by_reduction flags; the pair a_by_reduction = 0,
  * b_by_reduction = 1 is not offered (exchange A and B).  Any alignment of the element type is accepted; 16-byte aligned
@@ -542,7 +544,7 @@ enum { DH_F32 = 0, DH_F16 = 1, DH_BF16 = 2 };
 enum { DH_ACT_NONE = 0, DH_ACT_RELU = 1, DH_ACT_SILU = 2, DH_ACT_GELU = 3, DH_ACT_SIGMOID = 4, DH_ACT_LAST = 4 };
 typedef struct dh_product {
     const void *a, *b, *bias, *residual;
-    void *out, *z;
+    void *out, *z, *a_sum;
     int64_t lda, ldb, ldo, ldr;
     int64_t a_batch, b_batch, o_batch, res_batch;
     int I, J, R, batch;

@@ -107,6 +107,7 @@ struct Plan {               // one problem of a launch and how it is cut
     int first, count;       // first workgroup of this problem (a multiple of 8), and how many it has
     int stream;             // out and z are stored past the caches, in 16-byte pieces
     float* partial;         // split > 1: [split][out_batches][I][J]
+    float* partial_sum;     // split > 1 and a_sum: [split][I]
 };
 
 struct Launch {
@@ -321,8 +322,9 @@ struct Feed {
 };
 
 // One reduction step of a wave's tile from LDS.
+// `sums`: also add up A's rows, as a product with ones.
 template <typename T, typename TA, typename TB, int BR, int TI, int TJ>
-__device__ __forceinline__ void multiply(f4 (&acc)[TI][TJ], const T* la, const T* lb, int wi, int wj, int lane)
+__device__ __forceinline__ void multiply(f4 (&acc)[TI][TJ], f4 (&rows)[TI], bool sums, const T* la, const T* lb, int wi, int wj, int lane)
 {
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -339,8 +341,17 @@ __device__ __forceinline__ void multiply(f4 (&acc)[TI][TJ], const T* la, const T
 #pragma unroll
                     for (int b = 0; b < TJ; ++b)
                         acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[b][e], fa[a][e], acc[a][b], 0, 0, 0);
+            if (sums) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int a = 0; a < TI; ++a) rows[a] = __builtin_amdgcn_mfma_f32_16x16x4f32(1.f, fa[a][e], rows[a], 0, 0, 0);
+            }
         }
     } else {
+        s8 ones;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ones[e] = std::is_same<T, __bf16>::value ? 0x3F80 : 0x3C00;
 #pragma unroll
         for (int kk = 0; kk < BR / 32; ++kk) {
             s8 fa[TI], fb[TJ];
@@ -352,6 +363,10 @@ __device__ __forceinline__ void multiply(f4 (&acc)[TI][TJ], const T* la, const T
             for (int a = 0; a < TI; ++a)
 #pragma unroll
                 for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<T>(fb[b], fa[a], acc[a][b]);
+            if (sums) {
+#pragma unroll
+                for (int a = 0; a < TI; ++a) rows[a] = mma16<T>(ones, fa[a], rows[a]);
+            }
         }
     }
 }
@@ -382,6 +397,21 @@ __device__ __forceinline__ bool place(const Launch& L, int BI, int BJ, Place* at
     at->s = rest / q.out_batches;
     at->batch = rest - at->s * q.out_batches;
     return true;
+}
+
+// The sums of A's rows that a wave holds (every lane of a column has the row's), to the result or to the partial sums.
+template <typename T, int TI>
+__device__ __forceinline__ void row_sums(const f4 (&rows)[TI], const Plan& q, const Place& at, int i0)
+{
+    const int lane = threadIdx.x & 63;
+    if (lane >= 16) return;
+#pragma unroll
+    for (int a = 0; a < TI; ++a) {
+        const int i = i0 + 16 * a + lane;
+        if (i >= q.p.I) continue;
+        if (q.split > 1) q.partial_sum[(int64_t)at.s * q.p.I + i] = rows[a][0];
+        else ((T*)q.p.a_sum)[i] = Elem<T>::down(rows[a][0]);
+    }
 }
 
 // What happens to a wave's accumulators.  They hold C in squares (a lane has four consecutive j of one row), memory wants rows:
@@ -524,6 +554,10 @@ __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
     for (int a = 0; a < TI; ++a)
 #pragma unroll
         for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 rows[TI];
+#pragma unroll
+    for (int a = 0; a < TI; ++a) rows[a] = f4{0.f, 0.f, 0.f, 0.f};
+    const bool sums = p.a_sum && at.j0 + wj == 0;
 
     SA sa;
     SB sb;
@@ -561,10 +595,11 @@ __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
         else wait_and_meet<0>();
         if (asked < k_end) ask();
         const T* from = lds[(k - k_begin) % STAGES];
-        multiply<T, TA, TB, BR, TI, TJ>(acc, from, from + BI * BR, wi, wj, lane);
+        multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, from, from + BI * BR, wi, wj, lane);
     }
     static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
     __syncthreads();
+    if (sums) row_sums<T, TI>(rows, q, at, at.i0 + wi);
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
@@ -596,6 +631,10 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
     for (int a = 0; a < TI; ++a)
 #pragma unroll
         for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
+    f4 rows[TI];
+#pragma unroll
+    for (int a = 0; a < TI; ++a) rows[a] = f4{0.f, 0.f, 0.f, 0.f};
+    const bool sums = p.a_sum && at.j0 + wj == 0;
 
     int left = 0, batch = at.batch;
     auto enter = [&](int r0) {
@@ -627,10 +666,11 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
         FB::stage(lds_b, rb);
         __syncthreads();
         if (k + 1 < k_end) fetch();
-        multiply<T, TA, TB, BR, TI, TJ>(acc, lds_a, lds_b, wi, wj, lane);
+        multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, lds_a, lds_b, wi, wj, lane);
     }
     static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
     __syncthreads();
+    if (sums) row_sums<T, TI>(rows, q, at, at.i0 + wi);
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
@@ -734,18 +774,60 @@ __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
     finish_one<T>(p, L.act, ob, i, j, v);
 }
 
-// Sums the partial products of the workgroups along the reduction, in their order, and finishes them.
+// Sums the partial products of the workgroups along the reduction, in their order, and finishes them: four values per thread,
+// eight of their parts requested at a time.  All products of a launch that were split join in one launch.
+struct Joins {
+    int w[DH_MAX_PRODUCTS], first[DH_MAX_PRODUCTS + 1], n;
+};
 template <typename T>
-__global__ void __launch_bounds__(256) k_product_join(const Plan q, int act)
+__global__ void __launch_bounds__(256) k_product_join(const Launch L, const Joins js)
 {
+    int k = 0;
+    while (k + 1 < js.n && (int)blockIdx.x >= js.first[k + 1]) ++k;
+    const Plan& q = L.plan[js.w[k]];
     const dh_product& p = q.p;
-    const int64_t n = (int64_t)q.out_batches * p.I * p.J;
-    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int64_t n = (int64_t)q.out_batches * p.I * p.J, extra = p.a_sum ? p.I : 0;
+    const int64_t at = ((int64_t)((int)blockIdx.x - js.first[k]) * 256 + threadIdx.x) * 4;
+    if (at >= n) {                          // behind the products: the row sums, one per thread
+        const int64_t i = at / 4 - (n + 3) / 4;
+        if (i >= extra) return;
         float v = 0.f;
-        for (int s = 0; s < q.split; ++s) v += q.partial[(int64_t)s * n + k];
-        const int64_t rest = k / p.J;
-        const int j = (int)(k - rest * p.J), b = (int)(rest / p.I), i = (int)(rest - (int64_t)b * p.I);
-        finish_one<T>(p, act, b, i, j, v);
+        for (int s = 0; s < q.split; ++s) v += q.partial_sum[(int64_t)s * p.I + i];
+        ((T*)p.a_sum)[i] = Elem<T>::down(v);
+        return;
+    }
+    const float* from = q.partial + at;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (at + 4 <= n) {
+        int s = 0;
+        for (; s + 8 <= q.split; s += 8) {
+            f4 t[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) __builtin_memcpy(&t[u], from + (int64_t)(s + u) * n, 16);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v += t[u];
+        }
+        for (; s < q.split; ++s) {
+            f4 t;
+            __builtin_memcpy(&t, from + (int64_t)s * n, 16);
+            v += t;
+        }
+    } else {
+        for (int s = 0; s < q.split; ++s)
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+                if (at + e < n) v[e] += from[(int64_t)s * n + e];
+    }
+    int64_t rest = at / p.J;
+    int j = (int)(at - rest * p.J), b = (int)(rest / p.I), i = (int)(rest - (int64_t)b * p.I);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (at + e >= n) break;
+        finish_one<T>(p, L.act, b, i, j, v[e]);
+        if (++j == p.J) {
+            j = 0;
+            if (++i == p.I) { i = 0; ++b; }
+        }
     }
 }
 
@@ -777,7 +859,7 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
     }
     // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs
     const dh_product& p = ps[0];
-    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
+    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
         return Shape{0, 16, 128, 1};
     if (large < CUS) return Shape{64, 64, 128, 2};
     if (!aligned) return Shape{128, 128, 128, 1};
@@ -805,6 +887,17 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     const bool large = written > (32ll << 20);
     int64_t total = 0;
     size_t bytes = 0;
+    int64_t all_tiles = 0, tile_steps = 0;
+    for (int w = 0; w < n && t.bi; ++w) {
+        const dh_product& p = ps[w];
+        const int64_t tiles = (int64_t)((p.I + t.bi - 1) / t.bi) * ((p.J + t.bj - 1) / t.bj) * (p.reduce_batch ? 1 : p.batch);
+        all_tiles += tiles;
+        tile_steps += tiles * ((p.R + br - 1) / br) * (p.reduce_batch ? p.batch : 1);
+    }
+    const int64_t at_once = (int64_t)CUS * (t.bi == 256 ? 1 : t.bi == 64 ? 4 : t.stages == 3 ? 3 : 2);
+    const bool cutting = t.bi && all_tiles < at_once;
+    int64_t each = (tile_steps + at_once - 1) / at_once;
+    if (each < 4) each = 4;
     int order[DH_MAX_PRODUCTS];
     for (int w = 0; w < n; ++w) {          // long reductions first: their workgroups are the ones a launch waits for
         int k = w;
@@ -823,8 +916,10 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         const int64_t tiles = (int64_t)q.tiles_i * q.tiles_j * q.out_batches;
         if (steps >= (1ll << 31) || tiles >= (1ll << 28) || (int64_t)q.tiles_i * q.tiles_j >= (1ll << 27)) return DH_ERR_ARG;
         q.steps = (int)steps;
-        int64_t split = tiles >= 2 * CUS || tiles == 0 || t.bi == 0 ? 1 : (2 * CUS + tiles - 1) / tiles;
-        if (split > steps / 4) split = steps / 4;           // at least four steps each
+        // A reduction is cut so that all workgroups of the launch have about the same number of steps, four at least, and
+        // there are as many as run at one time.
+        int64_t split = 1;
+        if (cutting && tiles) split = (steps + each - 1) / each;
         if (split < 1) split = 1;
         q.per = (int)((steps + split - 1) / split);
         q.split = q.per ? (int)((steps + q.per - 1) / q.per) : 1;
@@ -833,6 +928,8 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         if (q.split > 1) {
             q.partial = (float*)((char*)ws + bytes);
             bytes += ((size_t)q.split * q.out_batches * p.I * p.J * sizeof(float) + 255) & ~(size_t)255;
+            q.partial_sum = (float*)((char*)ws + bytes);
+            if (p.a_sum) bytes += ((size_t)q.split * p.I * sizeof(float) + 255) & ~(size_t)255;
         }
         q.first = (int)total;
         q.count = (int)(tiles * q.split);
@@ -884,12 +981,20 @@ int launch(const Launch& L, bool arc, bool brc, bool aligned, const Shape& t, hi
         else if (arc) launch_tiles<T, true, false>(L, aligned, t, st);
         else launch_tiles<T, false, false>(L, aligned, t, st);
     }
-    for (int w = 0; w < L.n; ++w)
-        if (L.plan[w].split > 1) {
-            const int64_t n = (int64_t)L.plan[w].out_batches * L.plan[w].p.I * L.plan[w].p.J;
-            const int64_t blocks = (n + 255) / 256;
-            hipLaunchKernelGGL((k_product_join<T>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, L.plan[w], L.act);
-        }
+    Joins js;
+    js.n = 0;
+    int64_t blocks = 0;
+    for (int w = 0; w < L.n; ++w) {
+        const Plan& q = L.plan[w];
+        if (q.split <= 1) continue;
+        const int64_t n = (int64_t)q.out_batches * q.p.I * q.p.J, threads = (n + 3) / 4 + (q.p.a_sum ? q.p.I : 0);
+        js.w[js.n] = w;
+        js.first[js.n++] = (int)blocks;
+        blocks += (threads + 255) / 256;
+    }
+    js.first[js.n] = (int)blocks;
+    if (blocks >= (1ll << 31)) return DH_ERR_ARG;
+    if (js.n) hipLaunchKernelGGL((k_product_join<T>), dim3((unsigned)blocks), dim3(256), 0, st, L, js);
     return dh_launch_status();
 }
 
@@ -905,8 +1010,9 @@ int check(const dh_product* ps, int n, int dtype, int activation)
         if (!p.a_by_reduction && p.b_by_reduction) return DH_ERR_ARG;      // no caller has that pair
         const bool work = p.I > 0 && p.J > 0 && (p.reduce_batch || p.batch > 0);
         if (work && !p.out) return DH_ERR_ARG;
+        if (p.a_sum && ((!p.reduce_batch && p.batch != 1) || p.J < 1)) return DH_ERR_ARG;
         if (work && p.R > 0 && p.batch > 0 && (!p.a || !p.b)) return DH_ERR_ARG;
-        const uintptr_t all = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.z | (uintptr_t)p.residual | (uintptr_t)p.bias;
+        const uintptr_t all = (uintptr_t)p.a | (uintptr_t)p.b | (uintptr_t)p.out | (uintptr_t)p.z | (uintptr_t)p.residual | (uintptr_t)p.bias | (uintptr_t)p.a_sum;
         if (all % esize) return DH_ERR_ALIGN;
     }
     return DH_OK;

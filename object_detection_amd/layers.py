@@ -5,9 +5,11 @@
 
 Sums, bias, activation and residual are fp32 and the result is rounded once.  All three entries are differentiable (x, weight,
 bias, residual) and take fp32, fp16 or bf16 tensors of one type; under torch.autocast their inputs are cast to its type, as
-torch's own layers do.  A second derivative is not offered.
+torch's own layers do.  The backward of an activation reads the pre-activation, kept in the tensors' type.  A second derivative is
+not offered.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -20,25 +22,23 @@ MAX_PRODUCTS = 5
 
 class Product(ctypes.Structure):
     """Mirror of dh_product in include/dethead.h."""
-    _fields_ = ([(n, L.c_void_p) for n in ("a", "b", "bias", "residual", "out", "z")]
+    _fields_ = ([(n, L.c_void_p) for n in ("a", "b", "bias", "residual", "out", "z", "a_sum")]
                 + [(n, L.c_i64) for n in ("lda", "ldb", "ldo", "ldr", "a_batch", "b_batch", "o_batch", "res_batch")]
                 + [(n, L.c_int) for n in ("I", "J", "R", "batch", "a_by_reduction", "b_by_reduction", "bias_on_i", "reduce_batch")])
 
 
-def _address(t):
-    return t.data_ptr() if t is not None else 0
+# The same struct as bytes, its fields in order: a call fills it an order of magnitude faster than ctypes' attributes.
+_pack = struct.Struct("7Q8q8i").pack
+assert struct.calcsize("7Q8q8i") == ctypes.sizeof(Product)
 
 
 def _run(products, dtype, activation, device):
-    """One launch of the given products: dicts of tensors and geometry (see dh_product)."""
-    n = len(products)
-    table = (Product * n)(*[Product(**p) for p in products])
-    lib = L.lib()
-    code = _DTYPES[dtype]
+    """One launch of the given packed products."""
+    n, table, code, lib = len(products), b"".join(products), _DTYPES[dtype], L.lib()
     need = lib.dh_products_workspace(table, n, code)
     ws = L.workspace(need, device) if need else None
     with L.device_guard(device):
-        L.check(lib.dh_products(table, n, code, activation, L.ptr(ws), need, L.stream()), "dh_products")
+        L.check(lib.dh_products(table, n, code, activation, ws.data_ptr() if need else None, need, L.raw_stream()), "dh_products")
 
 
 def _slope(dy, z, activation, want_bias, outer, n, inner):
@@ -51,157 +51,186 @@ def _slope(dy, z, activation, want_bias, outer, n, inner):
     need = lib.dh_product_slope_workspace(n) if want_bias else 0
     ws = L.workspace(need, dy.device) if want_bias else None
     with L.device_guard(dy.device):
-        L.check(lib.dh_product_slope(L.ptr(dy), L.ptr(z), L.ptr(dz), L.ptr(dbias), outer, n, inner, activation, _DTYPES[dy.dtype],
-                                     L.ptr(ws), need, L.stream()), "dh_product_slope")
+        L.check(lib.dh_product_slope(dy.data_ptr(), z.data_ptr() if z is not None else None, dz.data_ptr(),
+                                     dbias.data_ptr() if want_bias else None, outer, n, inner, activation, _DTYPES[dy.dtype],
+                                     ws.data_ptr() if want_bias else None, need, L.raw_stream()), "dh_product_slope")
     return dz, dbias
 
 
-# ---- geometry: rows (M, K) -> (M, N) and maps (B, K, P) -> (B, N, P), both with the weight (N, K) ----
+# ---- layouts: rows (M, K) -> (M, N) and maps (B, K, ny, nx) -> (B, N, ny, nx), both with a dense weight of N x K ----
 
-def _rows_forward(x, w, bias, residual, out, z):
+def _as_rows(t):
+    """(..., C) -> (M, C) with the last axis dense and one stride between rows; a copy only where the strides do not allow a
+    view (or rows overlap, as in an expanded tensor)."""
+    t = t.reshape(t.shape[:-1].numel(), t.shape[-1]) if t.dim() != 2 else t
+    if not t.is_contiguous() and (t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _as_planes(t):
+    """(B, C, ny, nx) with dense planes, and the distance between its images: a slice of a wider tensor's channels is taken as
+    it is, anything else that is not dense is copied."""
+    if t.is_contiguous():
+        return t, t.shape[1] * t.shape[2] * t.shape[3]
+    b, c, h, w = t.shape
+    s = t.stride()
+    if s[1:] == (h * w, w, 1) and s[0] >= c * h * w:
+        return t, s[0]
+    return t.contiguous(), c * h * w
+
+
+def _rows_forward(x, w, bias, res, out, z):
     m, k = x.shape
-    return dict(a=_address(x), b=_address(w), bias=_address(bias), residual=_address(residual), out=_address(out), z=_address(z),
-                lda=x.stride(0), ldb=k, ldo=out.stride(0), ldr=residual.stride(0) if residual is not None else 0,
-                I=m, J=w.shape[0], R=k, batch=1, a_by_reduction=1, b_by_reduction=1)
-
-
-def _rows_grad_input(dz, w, out):
-    return dict(a=_address(dz), b=_address(w), out=_address(out), lda=dz.shape[1], ldb=w.shape[1], ldo=w.shape[1],
-                I=dz.shape[0], J=w.shape[1], R=dz.shape[1], batch=1, a_by_reduction=1, b_by_reduction=0)
-
-
-def _rows_grad_weight(dz, x, out):
-    return dict(a=_address(dz), b=_address(x), out=_address(out), lda=dz.shape[1], ldb=x.stride(0), ldo=x.shape[1],
-                I=dz.shape[1], J=x.shape[1], R=x.shape[0], batch=1, a_by_reduction=0, b_by_reduction=0)
-
-
-def _maps_forward(x, w, bias, residual, out, z):
-    b, k, p = x.shape
     n = w.shape[0]
-    return dict(a=_address(w), b=_address(x), bias=_address(bias), residual=_address(residual), out=_address(out), z=_address(z),
-                lda=k, ldb=p, ldo=p, ldr=p, b_batch=x.stride(0), o_batch=n * p,
-                res_batch=residual.stride(0) if residual is not None else 0,
-                I=n, J=p, R=k, batch=b, a_by_reduction=1, b_by_reduction=0, bias_on_i=1)
+    return _pack(x.data_ptr(), w.data_ptr(), bias.data_ptr() if bias is not None else 0, res.data_ptr() if res is not None else 0,
+                 out.data_ptr(), z.data_ptr() if z is not None else 0, 0, x.stride(0) if m > 1 else k, k, n,
+                 res.stride(0) if res is not None and m > 1 else n, 0, 0, 0, 0, m, n, k, 1, 1, 1, 0, 0)
 
 
-def _maps_grad_input(dz, w, out):
-    b, n, p = dz.shape
-    k = w.shape[1]
-    return dict(a=_address(w), b=_address(dz), out=_address(out), lda=k, ldb=p, ldo=p, b_batch=n * p, o_batch=k * p,
-                I=k, J=p, R=n, batch=b, a_by_reduction=0, b_by_reduction=0)
+def _maps_forward(x, x_batch, w, bias, res, res_batch, out, z):
+    b, k, h, v = x.shape
+    n, p = w.shape[0], h * v
+    return _pack(w.data_ptr(), x.data_ptr(), bias.data_ptr() if bias is not None else 0, res.data_ptr() if res is not None else 0,
+                 out.data_ptr(), z.data_ptr() if z is not None else 0, 0, k, p, p, p, 0, x_batch, n * p, res_batch, n, p, k, b, 1, 0, 1, 0)
 
 
-def _maps_grad_weight(dz, x, out):
-    b, n, p = dz.shape
-    k = x.shape[1]
-    return dict(a=_address(dz), b=_address(x), out=_address(out), lda=p, ldb=p, ldo=k, a_batch=n * p, b_batch=x.stride(0),
-                I=n, J=k, R=p, batch=b, a_by_reduction=1, b_by_reduction=1, reduce_batch=1)
+def _grad_input(rows, dz, w, out):
+    n, k = w.shape[0], w.shape[1]
+    if rows:
+        return _pack(dz.data_ptr(), w.data_ptr(), 0, 0, out.data_ptr(), 0, 0, n, k, k, 0, 0, 0, 0, 0, dz.shape[0], k, n, 1, 1, 0, 0, 0)
+    b, p = dz.shape[0], dz.shape[2] * dz.shape[3]
+    return _pack(w.data_ptr(), dz.data_ptr(), 0, 0, out.data_ptr(), 0, 0, k, p, p, 0, 0, n * p, k * p, 0, k, p, n, b, 0, 0, 0, 0)
 
 
-def _forward(rows, act, items, want_z):
-    """items: (x, w, bias, residual) with x (M, K) or (B, K, P) -> outputs, pre-activations."""
-    make = _rows_forward if rows else _maps_forward
-    x = items[0][0]
-    shape = (lambda x, w: (x.shape[0], w.shape[0])) if rows else (lambda x, w: (x.shape[0], w.shape[0], x.shape[2]))
-    outs = [torch.empty(shape(x, w), dtype=x.dtype, device=x.device) for x, w, _, _ in items]
-    zs = [torch.empty_like(o) if want_z else None for o in outs]
-    _run([make(x, w, b, r, o, z) for (x, w, b, r), o, z in zip(items, outs, zs)], x.dtype, act, x.device)
-    return outs, zs
+def _grad_weight(rows, dz, x, x_batch, out, dbias):
+    """With dbias: the bias gradient beside the weight's, from the same read of dz."""
+    k, n, db = x.shape[1], dz.shape[1], dbias.data_ptr() if dbias is not None else 0
+    if rows:
+        m = x.shape[0]
+        return _pack(dz.data_ptr(), x.data_ptr(), 0, 0, out.data_ptr(), 0, db, n, x.stride(0) if m > 1 else k, k, 0, 0, 0, 0, 0, n, k, m, 1,
+                     0, 0, 0, 0)
+    b, p = x.shape[0], x.shape[2] * x.shape[3]
+    return _pack(dz.data_ptr(), x.data_ptr(), 0, 0, out.data_ptr(), 0, db, p, p, k, 0, n * p, x_batch, 0, 0, n, k, p, b, 1, 1, 0, 1)
+
+
+def _forward(rows, act, items, keep):
+    """items: (x, weight, bias, residual), x (M, K) with `rows`, else (B, K, ny, nx) -> outputs; with keep also what a backward
+    needs, (x as it was read, pre-activation) of each."""
+    outs, kept, products, alive = [], [], [], []
+    for x, w, bias, res in items:
+        dtype, device, n = x.dtype, x.device, w.shape[0]
+        if not w.is_contiguous():
+            w = w.contiguous()
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
+        if rows:
+            x = _as_rows(x)
+            res = _as_rows(res) if res is not None else None
+            out = torch.empty((x.shape[0], n), dtype=dtype, device=device)
+        else:
+            x, x_batch = _as_planes(x)
+            res, res_batch = _as_planes(res) if res is not None else (None, 0)
+            out = torch.empty((x.shape[0], n, x.shape[2], x.shape[3]), dtype=dtype, device=device)
+        z = torch.empty_like(out) if keep and act else None
+        products.append(_rows_forward(x, w, bias, res, out, z) if rows else _maps_forward(x, x_batch, w, bias, res, res_batch, out, z))
+        outs.append(out)
+        kept += (x, w, z) if keep else ()
+        alive.append((x, w, bias, res))         # copies live until the launch is queued
+    _run(products, dtype, act, device)
+    return outs, kept
 
 
 class _Products(torch.autograd.Function):
-    """The products of one launch with their gradients.  tensors: x, w, bias, residual of each (bias, residual may be None)."""
+    """The products of one launch with their gradients.  tensors: x, weight, bias, residual of each (bias, residual may be None)."""
 
     @staticmethod
     def forward(ctx, rows, act, *tensors):
         items = [tensors[k:k + 4] for k in range(0, len(tensors), 4)]
-        outs, zs = _forward(rows, act, items, act != 0)
-        ctx.rows, ctx.act, ctx.n = rows, act, len(items)
-        ctx.save_for_backward(*[t for (x, w, _, _), z in zip(items, zs) for t in (x, w, z)])
+        outs, kept = _forward(rows, act, items, True)
+        ctx.rows, ctx.act = rows, act
+        ctx.save_for_backward(*kept)
         return tuple(outs)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
         rows, saved, wants = ctx.rows, ctx.saved_tensors, ctx.needs_input_grad
-        result, inputs, weights = [None, None], [], []
-        for k in range(ctx.n):
+        result, inputs, weights, alive = [None, None], [], [], []
+        for k, dy in enumerate(grads):
             x, w, z = saved[3 * k:3 * k + 3]
             want_x, want_w, want_b, want_r = wants[2 + 4 * k:6 + 4 * k]
-            dy = grads[k]
             dx = dw = db = None
             if dy is None:
                 result += [None] * 4
                 continue
             dy = dy.contiguous()
             if want_x or want_w or want_b:
-                outer, n, inner = (dy.shape[0], dy.shape[1], 1) if rows else dy.shape
-                dz, db = _slope(dy, z, ctx.act, want_b, outer, n, inner)
+                n, at_weight = dy.shape[1], z is None and want_w and x.shape[1] > 0
+                outer, inner = dy.shape[0], 1 if rows else dy.shape[2] * dy.shape[3]
+                # without an activation dy is dz: the weight's gradient reads it anyway and sums it for the bias
+                dz, db = (dy, torch.empty(n, dtype=dy.dtype, device=dy.device) if want_b else None) if at_weight else \
+                    _slope(dy, z, ctx.act, want_b, outer, n, inner)
                 if want_x:
                     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-                    inputs.append((_rows_grad_input if rows else _maps_grad_input)(dz, w, dx) | {"keep": dz})
+                    inputs.append(_grad_input(rows, dz, w, dx))
                 if want_w:
                     dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-                    weights.append((_rows_grad_weight if rows else _maps_grad_weight)(dz, x, dw) | {"keep": dz})
+                    weights.append(_grad_weight(rows, dz, x, 0 if rows else _as_planes(x)[1], dw, db if at_weight else None))
+                alive.append(dz)
             result += [dx, dw, db, dy if want_r else None]
-        keep = [p.pop("keep") for p in inputs + weights]
-        device = saved[0].device
         for group in (inputs, weights):
             if group:
-                _run(group, saved[0].dtype, 0, device)
-        del keep
+                _run(group, saved[0].dtype, 0, saved[0].device)
         return tuple(result)
 
 
 def _apply(rows, act, items):
-    tensors = [t for item in items for t in item]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return list(_Products.apply(rows, act, *tensors))
+    if torch.is_grad_enabled():
+        tensors = [t for item in items for t in item]
+        if any([t is not None and t.requires_grad for t in tensors]):
+            return _Products.apply(rows, act, *tensors)
     return _forward(rows, act, items, False)[0]
 
 
 def _activation(name, where):
-    if name not in ACTIVATIONS:
-        raise ValueError(f"{where}: activation must be one of {list(ACTIVATIONS)}, got {name!r}")
-    return ACTIVATIONS[name]
+    try:
+        return ACTIVATIONS[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"{where}: activation must be one of {list(ACTIVATIONS)}, got {name!r}") from None
 
 
 def _checked(where, x, weight, bias, residual):
-    """The tensors in one supported type on one ROCm device (cast to autocast's type where that is on)."""
-    tensors = [x, weight, bias, residual]
-    for t, name in zip(tensors, ("x", "weight", "bias", "residual")):
-        if t is None and name in ("bias", "residual"):
-            continue
+    """The four tensors, of one supported type on one ROCm device (cast to autocast's type where that is on)."""
+    tensors = [t for t in (x, weight, bias, residual) if t is not None]
+    for t in tensors:
         if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{where}: {name} must be a torch.Tensor, got {type(t).__name__}")
-        if not t.is_cuda:
-            raise RuntimeError(f"{where}: {name} is on {t.device}: object_detection_amd only runs on ROCm devices (no CPU fallback)")
-        if t.device != x.device:
-            raise RuntimeError(f"{where}: {name} is on {t.device}, x on {x.device}")
+            raise TypeError(f"{where}: expected torch.Tensor, got {type(t).__name__}")
+    if x is None or weight is None:
+        raise TypeError(f"{where}: x and weight must be tensors")
+    device = x.get_device()
+    if device < 0 or not x.is_cuda:
+        raise RuntimeError(f"{where}: x is on {x.device}: object_detection_amd only runs on ROCm devices (no CPU fallback)")
+    for t in tensors:
+        if t.get_device() != device:
+            raise RuntimeError(f"{where}: tensors on {t.device} and {x.device}")
     if torch.is_autocast_enabled("cuda"):
-        dtype = torch.get_autocast_dtype("cuda")
-        tensors = [t.to(dtype) if t is not None and t.is_floating_point() else t for t in tensors]
-    for t, name in zip(tensors, ("x", "weight", "bias", "residual")):
-        if t is not None and (t.dtype != tensors[0].dtype or t.dtype not in _DTYPES):
-            raise RuntimeError(f"{where}: x, weight, bias and residual must have one type, fp32, fp16 or bf16; {name} is {t.dtype}, "
-                               f"x {tensors[0].dtype}")
-    return tensors
+        to = torch.get_autocast_dtype("cuda")
+        x, weight, bias, residual = [t.to(to) if t is not None and t.is_floating_point() else t for t in (x, weight, bias, residual)]
+        tensors = [t for t in (x, weight, bias, residual) if t is not None]
+    dtype = x.dtype
+    for t in tensors:
+        if t.dtype != dtype or dtype not in _DTYPES:
+            raise RuntimeError(f"{where}: x, weight, bias and residual must have one type, fp32, fp16 or bf16; got {t.dtype} and {dtype}")
+    return x, weight, bias, residual
 
 
 def _check_weight(where, weight, bias, inputs):
-    if weight.dim() not in (2, 4) or (weight.dim() == 4 and weight.shape[2:] != (1, 1)) or weight.shape[1] != inputs:
-        raise RuntimeError(f"{where}: weight must be (outputs, {inputs}) or (outputs, {inputs}, 1, 1), got {tuple(weight.shape)}")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise RuntimeError(f"{where}: bias must be ({weight.shape[0]},), got {tuple(bias.shape)}")
-
-
-def _as_rows(t):
-    """(..., C) -> (M, C) with the last axis dense and one stride between rows; a copy only where the strides do not allow a
-    view (or rows overlap, as in an expanded tensor)."""
-    t = t.reshape(t.shape[:-1].numel(), t.shape[-1]) if t.dim() != 2 else t
-    if t.shape[-1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        t = t.contiguous()
-    return t
+    shape = weight.shape
+    if len(shape) not in (2, 4) or shape[1] != inputs or (len(shape) == 4 and shape[2:] != (1, 1)):
+        raise RuntimeError(f"{where}: weight must be (outputs, {inputs}) or (outputs, {inputs}, 1, 1), got {tuple(shape)}")
+    if bias is not None and bias.shape != shape[:1]:
+        raise RuntimeError(f"{where}: bias must be ({shape[0]},), got {tuple(bias.shape)}")
 
 
 def linear(x, weight, bias=None, activation=None, residual=None):
@@ -214,25 +243,13 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     if x.dim() < 1 or weight.dim() != 2:
         raise RuntimeError(f"linear: x must be (..., C) and weight (N, C), got {tuple(x.shape)} and {tuple(weight.shape)}")
     _check_weight("linear", weight, bias, x.shape[-1])
-    shape = x.shape[:-1] + weight.shape[:1]
-    if residual is not None:
-        if residual.shape != shape:
-            raise RuntimeError(f"linear: residual must be {tuple(shape)}, got {tuple(residual.shape)}")
-        residual = _as_rows(residual)
-    out, = _apply(True, act, [(_as_rows(x), weight.contiguous(), bias.contiguous() if bias is not None else None, residual)])
-    return out.view(shape)
-
-
-def _planes(t):
-    """(B, C, ny, nx) -> (B, C, P) with dense planes; images may be apart (a slice of a wider tensor)."""
-    b, c, h, w = t.shape
-    if t.stride()[1:] == (h * w, w, 1) and t.stride(0) >= c * h * w:
-        return t.view(b, c, h * w) if t.is_contiguous() else t.as_strided((b, c, h * w), (t.stride(0), h * w, 1))
-    return t.contiguous().view(b, c, h * w)
-
-
-def _channels_last(t):
-    return t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last) and not t.is_contiguous()
+    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
+        raise RuntimeError(f"linear: residual must be {tuple(x.shape[:-1] + weight.shape[:1])}, got {tuple(residual.shape)}")
+    if x.dim() == 2:
+        return _apply(True, act, [(x, weight, bias, residual)])[0]
+    rows, n = x.shape[:-1].numel(), weight.shape[0]
+    out = _apply(True, act, [(x.reshape(rows, x.shape[-1]), weight, bias, residual.reshape(rows, n) if residual is not None else None)])[0]
+    return out.view(x.shape[:-1] + (n,))
 
 
 def pointwise_conv(x, weight, bias=None, activation=None, residual=None):
@@ -249,23 +266,11 @@ def pointwise_conv(x, weight, bias=None, activation=None, residual=None):
     n = weight.shape[0]
     if residual is not None and residual.shape != (b, n, h, w):
         raise RuntimeError(f"pointwise_conv: residual must be {(b, n, h, w)}, got {tuple(residual.shape)}")
-    weight = weight.reshape(n, c).contiguous()
-    bias = bias.contiguous() if bias is not None else None
-    if _channels_last(x):
-        rows = x.permute(0, 2, 3, 1).reshape(-1, c)
-        res = _as_rows(residual.permute(0, 2, 3, 1).reshape(-1, n)) if residual is not None else None
-        out, = _apply(True, act, [(rows, weight, bias, res)])
+    if not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last):
+        res = residual.permute(0, 2, 3, 1).reshape(b * h * w, n) if residual is not None else None
+        out = _apply(True, act, [(x.permute(0, 2, 3, 1).reshape(b * h * w, c), weight, bias, res)])[0]
         return out.view(b, h, w, n).permute(0, 3, 1, 2)
-    out, = _apply(False, act, [(_dense(x), weight, bias, _dense(residual) if residual is not None else None)])
-    return out.view(b, n, h, w)
-
-
-def _dense(t):
-    """_planes() through autograd: torch's own view operations where a gradient has to find its way back."""
-    if t.requires_grad and torch.is_grad_enabled():
-        b, c, h, w = t.shape
-        return t.reshape(b, c, h * w) if t.is_contiguous() else t.contiguous().view(b, c, h * w)
-    return _planes(t)
+    return _apply(False, act, [(x, weight, bias, residual)])[0]
 
 
 def head_convs(xs, weights, biases):
@@ -274,14 +279,13 @@ def head_convs(xs, weights, biases):
     xs, weights, biases = list(xs), list(weights), list(biases)
     if not xs or len(xs) > MAX_PRODUCTS or len(weights) != len(xs) or len(biases) != len(xs):
         raise RuntimeError(f"head_convs: 1 to {MAX_PRODUCTS} levels with a weight and a bias each, got {len(xs)}, {len(weights)}, {len(biases)}")
-    items, shapes = [], []
-    for l, (x, weight, bias) in enumerate(zip(xs, weights, biases)):
-        x, weight, bias, _ = _checked(f"head_convs, level {l}", x, weight, bias, None)
+    items = []
+    for x, weight, bias in zip(xs, weights, biases):
+        x, weight, bias, _ = _checked("head_convs", x, weight, bias, None)
         if x.dim() != 4:
-            raise RuntimeError(f"head_convs, level {l}: x must be (B, C, ny, nx), got {tuple(x.shape)}")
-        _check_weight(f"head_convs, level {l}", weight, bias, x.shape[1])
-        if items and (x.dtype != items[0][0].dtype or x.device != items[0][0].device):
-            raise RuntimeError(f"head_convs, level {l}: {x.dtype} on {x.device}, level 0 {items[0][0].dtype} on {items[0][0].device}")
-        items.append((_dense(x), weight.reshape(weight.shape[0], -1).contiguous(), bias.contiguous() if bias is not None else None, None))
-        shapes.append((x.shape[0], weight.shape[0]) + tuple(x.shape[2:]))
-    return [o.view(s) for o, s in zip(_apply(False, 0, items), shapes)]
+            raise RuntimeError(f"head_convs, level {len(items)}: x must be (B, C, ny, nx), got {tuple(x.shape)}")
+        _check_weight("head_convs", weight, bias, x.shape[1])
+        if items and (x.dtype != items[0][0].dtype or x.get_device() != items[0][0].get_device()):
+            raise RuntimeError(f"head_convs, level {len(items)}: {x.dtype} on {x.device}, level 0 {items[0][0].dtype} on {items[0][0].device}")
+        items.append((x, weight, bias, None))
+    return list(_apply(False, 0, items))

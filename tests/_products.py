@@ -35,7 +35,8 @@ def act64(z, name):
 
 
 def rows64(x, w, bias, act, residual, dy=None):
-    """Values and bounds of one product over rows; x (M, K), w (N, K), everything on the CPU.  Returns {name: (value, bound)}."""
+    """Values and bounds of one product over rows; x (M, K), w (N, K), on the device the tensors are on.  Returns {name: (value,
+    bound)}."""
     dtype = x.dtype
     ut, low = half_step(dtype), LOWEST[dtype]
     X, W = x.double(), w.double()
@@ -74,7 +75,7 @@ def rows64(x, w, bias, act, residual, dy=None):
 
 def close(got, want, label=""):
     value, bound = want
-    got = got.detach().double().cpu().reshape(value.shape)
+    got = got.detach().to(value.device).double().reshape(value.shape)
     off = (got - value).abs()
     bad = ~(off <= bound)
     if bad.any():

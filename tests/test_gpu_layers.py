@@ -122,6 +122,46 @@ def test_maps_channels_last(dtype):
     assert y.is_contiguous(memory_format=torch.channels_last)
 
 
+# Sizes that reach every tile shape (128 x 128 in both step lengths, 256 x 256, the thin kernel's one and two row blocks, split
+# reductions of each), with edges that fill no tile; the 64-bit side runs on the GPU.
+LARGE = [(4100, 136, 1040, "silu", True), (4100, 1048, 1040, "gelu", False), (8200, 520, 4080, None, True), (16, 4096, 2056, "silu", True),
+         (17, 2056, 2100, "gelu", True), (32, 520, 4096, None, False), (5, 1001, 2049, "silu", True), (700, 8192, 72, "silu", True),
+         (3001, 333, 1501, "silu", True)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n,act,residual", LARGE)
+def test_rows_every_shape(m, k, n, act, residual, dtype):
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = [t.cuda() for t in rows_case(m, k, n, dtype, act, True, True, seed=3)]
+    r = r if residual else None
+    want = rows64(x, w, b, act, r, dy)
+    gx, gw, gb = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    y = linear(gx, gw, gb, act, r)
+    close(y, want["y"], "y")
+    y.backward(dy)
+    close(gx.grad, want["dx"], "dx")
+    close(gw.grad, want["dw"], "dw")
+    close(gb.grad, want["db"], "db")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,k,n,ny,nx,act", [(8, 128, 255, 80, 80, None), (6, 72, 250, 52, 52, "silu"), (4, 512, 512, 52, 64, None),
+                                             (3, 100, 260, 75, 61, "gelu"), (130, 40, 264, 13, 13, "silu")])
+def test_maps_every_shape(b, k, n, ny, nx, act, dtype):
+    from object_detection_amd.layers import pointwise_conv
+    x, w, bias = made((b, k, ny, nx), dtype, 1).cuda(), made((n, k, 1, 1), dtype, 2, k ** -0.5).cuda(), made((n,), dtype, 3, 0.5).cuda()
+    r, dy = made((b, n, ny, nx), dtype, 4).cuda(), made((b, n, ny, nx), dtype, 5).cuda()
+    want = rows64(to_rows(x), w.reshape(n, k), bias, act, to_rows(r), to_rows(dy))
+    gx, gw, gb = [t.clone().requires_grad_(True) for t in (x, w, bias)]
+    y = pointwise_conv(gx, gw, gb, act, r)
+    close(to_rows(y), want["y"], "y")
+    y.backward(dy)
+    close(to_rows(gx.grad), want["dx"], "dx")
+    close(gw.grad.reshape(n, k), want["dw"], "dw")
+    close(gb.grad, want["db"], "db")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_head_levels(dtype):
     """Three levels of different widths and sizes in one launch; one level without a bias."""
