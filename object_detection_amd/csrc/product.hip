@@ -603,8 +603,8 @@ __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
-// Any alignment: one buffer in LDS behind one step in registers.
-template <typename T, int BI, int BJ, int BR, int WI, int WJ, bool ARC, bool BRC>
+// Any alignment: one buffer in LDS behind DEPTH steps on their way in registers.
+template <typename T, int BI, int BJ, int BR, int WI, int WJ, int DEPTH, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
 {
     constexpr int THREADS = WI * WJ * 64;
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
     const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
     FA feed_a;
     FB feed_b;
-    u4 ra[FA::N], rb[FB::N];
+    u4 ra[DEPTH][FA::N], rb[DEPTH][FB::N];
     f4 acc[TI][TJ];
 #pragma unroll
     for (int a = 0; a < TI; ++a)
@@ -650,23 +650,29 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
         }
         enter(r * BR);
     }
-    auto fetch = [&]() {
+    auto fetch = [&](int d) {
         if (left <= 0) {
             ++batch;
             enter(0);
         }
-        feed_a.fetch(ra, left);
-        feed_b.fetch(rb, left);
+        feed_a.fetch(ra[d], left);
+        feed_b.fetch(rb[d], left);
         left -= BR;
     };
-    if (k_begin < k_end) fetch();
-    for (int k = k_begin; k < k_end; ++k) {
-        __syncthreads();
-        FA::stage(lds_a, ra);
-        FB::stage(lds_b, rb);
-        __syncthreads();
-        if (k + 1 < k_end) fetch();
-        multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, lds_a, lds_b, wi, wj, lane);
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (k_begin + d < k_end) fetch(d);
+    for (int k = k_begin; k < k_end; k += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            if (k + d >= k_end) break;
+            __syncthreads();
+            FA::stage(lds_a, ra[d]);
+            FB::stage(lds_b, rb[d]);
+            __syncthreads();
+            if (k + d + DEPTH < k_end) fetch(d);
+            multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, lds_a, lds_b, wi, wj, lane);
+        }
     }
     static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
     __syncthreads();
@@ -774,49 +780,60 @@ __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
     finish_one<T>(p, L.act, ob, i, j, v);
 }
 
-// Sums the partial products of the workgroups along the reduction, in their order, and finishes them: four values per thread,
-// eight of their parts requested at a time.  All products of a launch that were split join in one launch.
+// Sums the partial products of the workgroups along the reduction, in a fixed order, and finishes them.  A thread adds four
+// values' parts, eight requested at a time; with many parts, eight threads share them (every eighth part each) and their sums are
+// added in turn.  All products of a launch that were split join in one launch.
 struct Joins {
     int w[DH_MAX_PRODUCTS], first[DH_MAX_PRODUCTS + 1], n;
+    int share[DH_MAX_PRODUCTS];             // 1 or 8 threads per value
 };
 template <typename T>
 __global__ void __launch_bounds__(256) k_product_join(const Launch L, const Joins js)
 {
+    __shared__ f4 shared[256];
     int k = 0;
     while (k + 1 < js.n && (int)blockIdx.x >= js.first[k + 1]) ++k;
     const Plan& q = L.plan[js.w[k]];
     const dh_product& p = q.p;
-    const int64_t n = (int64_t)q.out_batches * p.I * p.J, extra = p.a_sum ? p.I : 0;
-    const int64_t at = ((int64_t)((int)blockIdx.x - js.first[k]) * 256 + threadIdx.x) * 4;
-    if (at >= n) {                          // behind the products: the row sums, one per thread
-        const int64_t i = at / 4 - (n + 3) / 4;
-        if (i >= extra) return;
-        float v = 0.f;
-        for (int s = 0; s < q.split; ++s) v += q.partial_sum[(int64_t)s * p.I + i];
-        ((T*)p.a_sum)[i] = Elem<T>::down(v);
-        return;
-    }
-    const float* from = q.partial + at;
+    const int share = js.share[k], wide = 256 / share, part = (int)threadIdx.x / wide;
+    const int64_t n = (int64_t)q.out_batches * p.I * p.J, quads = (n + 3) / 4;
+    const int64_t quad = (int64_t)((int)blockIdx.x - js.first[k]) * wide + threadIdx.x % wide, at = quad * 4;
+    const bool products = quad < quads;
     f4 v = {0.f, 0.f, 0.f, 0.f};
-    if (at + 4 <= n) {
-        int s = 0;
-        for (; s + 8 <= q.split; s += 8) {
-            f4 t[8];
+    if (products) {
+        const float* from = q.partial + at;
+        if (at + 4 <= n) {
+            int s = part;
+            for (; s + 7 * share < q.split; s += 8 * share) {
+                f4 t[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) __builtin_memcpy(&t[u], from + (int64_t)(s + u) * n, 16);
+                for (int u = 0; u < 8; ++u) __builtin_memcpy(&t[u], from + (int64_t)(s + u * share) * n, 16);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v += t[u];
+                for (int u = 0; u < 8; ++u) v += t[u];
+            }
+            for (; s < q.split; s += share) {
+                f4 t;
+                __builtin_memcpy(&t, from + (int64_t)s * n, 16);
+                v += t;
+            }
+        } else {
+            for (int s = part; s < q.split; s += share)
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (at + e < n) v[e] += from[(int64_t)s * n + e];
         }
-        for (; s < q.split; ++s) {
-            f4 t;
-            __builtin_memcpy(&t, from + (int64_t)s * n, 16);
-            v += t;
-        }
-    } else {
-        for (int s = 0; s < q.split; ++s)
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-                if (at + e < n) v[e] += from[(int64_t)s * n + e];
+    } else if (p.a_sum && quad - quads < p.I) {       // behind the products: the row sums, one each
+        for (int s = part; s < q.split; s += share) v[0] += q.partial_sum[(int64_t)s * p.I + quad - quads];
+    }
+    if (share > 1) {                        // uniform in the workgroup
+        shared[threadIdx.x] = v;
+        __syncthreads();
+        if (part) return;
+        for (int u = 1; u < share; ++u) v += shared[u * wide + threadIdx.x];
+    }
+    if (!products) {
+        if (p.a_sum && quad - quads < p.I) ((T*)p.a_sum)[quad - quads] = Elem<T>::down(v[0]);
+        return;
     }
     int64_t rest = at / p.J;
     int j = (int)(at - rest * p.J), b = (int)(rest / p.I), i = (int)(rest - (int64_t)b * p.I);
@@ -845,26 +862,32 @@ struct Shape { int bi, bj, br, stages; };        // br: bytes of a reduction ste
 //   128 x 128 in steps of 128 bytes and 2 stages where the reduction is long: 8192 x 4096 -> 1024 66 against 78; in steps of 64
 //     bytes and 3 stages (48 KB: three workgroups per CU) where it is short and loading, multiplying and storing have to
 //     overlap between workgroups: the head's levels (128 to 512 channels) at batch 64 119 against 159.
-//   64 x 64 where 128 x 128 would leave CUs without a tile.
+//   64 x 64 where 128 x 128 would leave CUs without a tile, unless the reduction can be cut into 16 or more steps for two
+//     workgroups per CU: the head's weight gradients at batch 64 (14 tiles, 44 steps each) 117 against 155, 1024 x 1024 over 8192 rows
+//     (16 steps) 34 against 45; but 128 x 128 over 64 x 80 x 80 cells (12 steps) 56 against 40.
 Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
 {
-    int64_t huge = 0, large = 0, held = 0;
-    int longest = 0;
+    int64_t huge = 0, large = 0, held = 0, tile_steps = 0;
+    const int64_t br = dtype == DH_F32 ? 32 : 64;
+    int longest = 0, shortest = 1 << 30;
     for (int w = 0; w < n; ++w) {
         const int64_t b = ps[w].reduce_batch ? 1 : ps[w].batch;
         huge += (int64_t)((ps[w].I + 255) / 256) * ((ps[w].J + 255) / 256) * b;
-        large += (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * b;
+        const int64_t tiles = (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * b;
+        large += tiles;
+        tile_steps += tiles * ((ps[w].R + br - 1) / br) * (ps[w].reduce_batch ? ps[w].batch : 1);
         held += (int64_t)ps[w].I * ps[w].J * b;
         if (ps[w].R > longest) longest = ps[w].R;
+        if (ps[w].R < shortest) shortest = ps[w].R;
     }
     // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs
     const dh_product& p = ps[0];
     if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
         return Shape{0, 16, 128, 1};
-    if (large < CUS) return Shape{64, 64, 128, 2};
+    if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, 2};
     if (!aligned) return Shape{128, 128, 128, 1};
-    if (dtype != DH_F32 && huge >= 2 * CUS && longest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
-    return longest >= 1024 ? Shape{128, 128, 128, 2} : Shape{128, 128, 64, 3};
+    if (dtype != DH_F32 && huge >= 2 * CUS && shortest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
+    return longest >= 1024 || large < CUS ? Shape{128, 128, 128, 2} : Shape{128, 128, 64, 3};
 }
 
 int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws_bytes, bool* aligned, Shape* shape)
@@ -894,10 +917,11 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         all_tiles += tiles;
         tile_steps += tiles * ((p.R + br - 1) / br) * (p.reduce_batch ? p.batch : 1);
     }
-    const int64_t at_once = (int64_t)CUS * (t.bi == 256 ? 1 : t.bi == 64 ? 4 : t.stages == 3 ? 3 : 2);
-    const bool cutting = t.bi && all_tiles < at_once;
-    int64_t each = (tile_steps + at_once - 1) / at_once;
-    if (each < 4) each = 4;
+    // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
+    // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each.
+    const bool cutting = t.bi && all_tiles < CUS;
+    int64_t each = (tile_steps + 2 * CUS - 1) / (2 * CUS);
+    if (each < 1024 / t.br) each = 1024 / t.br;
     int order[DH_MAX_PRODUCTS];
     for (int w = 0; w < n; ++w) {          // long reductions first: their workgroups are the ones a launch waits for
         int k = w;
@@ -916,8 +940,6 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         const int64_t tiles = (int64_t)q.tiles_i * q.tiles_j * q.out_batches;
         if (steps >= (1ll << 31) || tiles >= (1ll << 28) || (int64_t)q.tiles_i * q.tiles_j >= (1ll << 27)) return DH_ERR_ARG;
         q.steps = (int)steps;
-        // A reduction is cut so that all workgroups of the launch have about the same number of steps, four at least, and
-        // there are as many as run at one time.
         int64_t split = 1;
         if (cutting && tiles) split = (steps + each - 1) / each;
         if (split < 1) split = 1;
@@ -969,8 +991,8 @@ void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
 #undef DH_CASE
         return;
     }
-    if (t.bi == 128) hipLaunchKernelGGL((k_product_any<T, 128, 128, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
-    else hipLaunchKernelGGL((k_product_any<T, 64, 64, BR, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
+    if (t.bi == 128) hipLaunchKernelGGL((k_product_any<T, 128, 128, BR, 2, 2, 1, ARC, BRC>), grid, dim3(256), 0, st, L);
+    else hipLaunchKernelGGL((k_product_any<T, 64, 64, BR, 2, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
 }
 
 template <typename T>
@@ -988,9 +1010,11 @@ int launch(const Launch& L, bool arc, bool brc, bool aligned, const Shape& t, hi
         const Plan& q = L.plan[w];
         if (q.split <= 1) continue;
         const int64_t n = (int64_t)q.out_batches * q.p.I * q.p.J, threads = (n + 3) / 4 + (q.p.a_sum ? q.p.I : 0);
+        const int share = q.split >= 32 ? 8 : 1;
         js.w[js.n] = w;
+        js.share[js.n] = share;
         js.first[js.n++] = (int)blocks;
-        blocks += (threads + 255) / 256;
+        blocks += (threads * share + 255) / 256;
     }
     js.first[js.n] = (int)blocks;
     if (blocks >= (1ll << 31)) return DH_ERR_ARG;
@@ -1019,66 +1043,121 @@ int check(const dh_product* ps, int n, int dtype, int activation)
 }
 
 // ---- dz = dy * act'(z) and the bias gradient ----
-// dy is [outer][n][inner]; the bias gradient sums over outer and inner.  SPLIT workgroups share one n (inner > 1) or one
-// column block (inner == 1); their sums go to the workspace and are added in order by k_bias_join.
-constexpr int BIAS_SPLIT = 64;
+// dy is [outer][n][inner]; the bias gradient sums over outer and inner.  One pass over dy and z in 16-byte pieces (of any
+// alignment): a wave takes rows of `inner` values of one n (maps), or the same 64 pieces of columns in every row (inner = 1).
+// Sums go to the workspace, SPLIT of them at most per n, and are added in order by k_bias_join.
+constexpr int BIAS_SPLIT = 256;
 
-template <typename T> __device__ __forceinline__ float slope_of(float z, int act)
+// v[k] = dy * act'(z), stored where dz is; the values count from `at` in one piece of V, `n` of them exist
+template <typename T, int V>
+__device__ __forceinline__ void slope_piece(const T* dy, const T* z, T* dz, int64_t at, int n, int act, float* v)
 {
-    float v = 1.f;
-    with_act(act, [&](auto a) { v = Act<decltype(a)::value, sizeof(T) == 2>::slope(z); });
-    return v;
+    T g[V], y[V];
+    const bool whole = n >= V;
+    if (whole) {
+        __builtin_memcpy(g, dy + at, 16);
+        if (z) __builtin_memcpy(y, z + at, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            g[k] = k < n ? dy[at + k] : T(0);
+            y[k] = z && k < n ? z[at + k] : T(0);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = Elem<T>::up(g[k]);
+    if (!z) return;
+    with_act(act, [&](auto a) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] *= Act<decltype(a)::value, sizeof(T) == 2>::slope(Elem<T>::up(y[k]));
+    });
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = Elem<T>::down(v[k]);
+    if (whole) {
+        __builtin_memcpy(dz + at, g, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (k < n) {
+                dz[at + k] = g[k];
+            } else {
+                v[k] = 0.f;         // (dy is 0 there, but the slope at 0 need not be finite times 0)
+            }
+    }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) k_slope_planes(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
-                                                      float* __restrict__ partial, int64_t outer, int64_t n, int64_t inner, int act)
+                                                      float* __restrict__ partial, int64_t outer, int64_t n, int64_t inner, int act, int split)
 {
-    const int64_t c = blockIdx.x / BIAS_SPLIT, s = blockIdx.x % BIAS_SPLIT;
+    constexpr int V = Elem<T>::CH;
+    const int64_t c = blockIdx.x % n, s = blockIdx.x / n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float sum = 0.f;
-    for (int64_t o = s; o < outer; o += BIAS_SPLIT) {
-        const int64_t at = (o * n + c) * inner;
-        for (int64_t k = threadIdx.x; k < inner; k += 256) {
-            float g = Elem<T>::up(dy[at + k]);
-            if (z) { g *= slope_of<T>(Elem<T>::up(z[at + k]), act); dz[at + k] = Elem<T>::down(g); }
-            sum += g;
+    for (int64_t o = s * 4 + wave; o < outer; o += 4 * split) {
+        const int64_t row = (o * n + c) * inner;
+#pragma unroll 4
+        for (int64_t k = lane * V; k < inner; k += 64 * V) {
+            float v[V];
+            slope_piece<T, V>(dy, z, dz, row + k, inner - k < V ? (int)(inner - k) : V, act, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += v[e];
         }
     }
     if (!partial) return;
     __shared__ float sums[4];
     sum = dh_wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+    if (lane == 0) sums[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0) partial[s * n + c] = sums[0] + sums[1] + sums[2] + sums[3];
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) k_slope_rows(const T* __restrict__ dy, const T* __restrict__ z, T* __restrict__ dz,
-                                                    float* __restrict__ partial, int64_t rows, int64_t n, int act)
+                                                    float* __restrict__ partial, int64_t rows, int64_t n, int act, int split)
 {
-    const int64_t c = (blockIdx.x / BIAS_SPLIT) * 64 + (threadIdx.x & 63), s = blockIdx.x % BIAS_SPLIT;
-    float sum = 0.f;
+    constexpr int V = Elem<T>::CH;
+    __shared__ float sums[4][64 * V];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t columns = (n + 64 * V - 1) / (64 * V);
+    const int64_t c = blockIdx.x % columns * 64 * V + lane * V, s = blockIdx.x / columns;
+    const int here = n - c < V ? (int)(n - c) : V;
+    float sum[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sum[e] = 0.f;
     if (c < n)
-        for (int64_t r = s * 4 + (threadIdx.x >> 6); r < rows; r += 4 * BIAS_SPLIT) {
-            float g = Elem<T>::up(dy[r * n + c]);
-            if (z) { g *= slope_of<T>(Elem<T>::up(z[r * n + c]), act); dz[r * n + c] = Elem<T>::down(g); }
-            sum += g;
+#pragma unroll 4
+        for (int64_t r = s * 4 + wave; r < rows; r += 4 * split) {
+            float v[V];
+            slope_piece<T, V>(dy, z, dz, r * n + c, here, act, v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[e] += v[e];
         }
     if (!partial) return;
-    __shared__ float sums[256];
-    sums[threadIdx.x] = sum;
+#pragma unroll
+    for (int e = 0; e < V; ++e) sums[wave][lane * V + e] = sum[e];
     __syncthreads();
-    if (threadIdx.x < 64 && c < n)
-        partial[s * n + c] = sums[threadIdx.x] + sums[threadIdx.x + 64] + sums[threadIdx.x + 128] + sums[threadIdx.x + 192];
+    for (int k = threadIdx.x; k < 64 * V; k += 256) {
+        const int64_t at = blockIdx.x % columns * 64 * V + k;
+        if (at < n) partial[s * n + at] = sums[0][k] + sums[1][k] + sums[2][k] + sums[3][k];
+    }
 }
 
+// 32 sums per workgroup, eight threads for each
 template <typename T>
-__global__ void __launch_bounds__(256) k_bias_join(const float* __restrict__ partial, T* __restrict__ dbias, int64_t n)
+__global__ void __launch_bounds__(256) k_bias_join(const float* __restrict__ partial, T* __restrict__ dbias, int64_t n, int split)
 {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= n) return;
+    __shared__ float shared[256];
+    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int part = threadIdx.x >> 5;
     float sum = 0.f;
-    for (int s = 0; s < BIAS_SPLIT; ++s) sum += partial[s * n + c];
+    if (c < n)
+#pragma unroll 4
+        for (int s = part; s < split; s += 8) sum += partial[s * n + c];
+    shared[threadIdx.x] = sum;
+    __syncthreads();
+    if (part || c >= n) return;
+    for (int u = 1; u < 8; ++u) sum += shared[u * 32 + threadIdx.x];
     dbias[c] = Elem<T>::down(sum);
 }
 
@@ -1087,14 +1166,20 @@ int launch_slope(const void* dy, const void* z, void* dz, void* dbias, int64_t o
                  float* ws, hipStream_t st)
 {
     float* partial = dbias ? ws : nullptr;
+    // about 2048 workgroups, each with four rows or more
+    const int64_t columns = inner > 1 ? n : (n + 64 * Elem<T>::CH - 1) / (64 * Elem<T>::CH);
+    int64_t split = (2048 + columns - 1) / columns;
+    if (split > (outer + 3) / 4) split = (outer + 3) / 4;
+    if (split > BIAS_SPLIT) split = BIAS_SPLIT;
+    if (split < 1) split = 1;
     if (inner > 1)
-        hipLaunchKernelGGL((k_slope_planes<T>), dim3((unsigned)(n * BIAS_SPLIT)), dim3(256), 0, st, (const T*)dy, (const T*)z, (T*)dz,
-                           partial, outer, n, inner, act);
+        hipLaunchKernelGGL((k_slope_planes<T>), dim3((unsigned)(columns * split)), dim3(256), 0, st, (const T*)dy, (const T*)z, (T*)dz,
+                           partial, outer, n, inner, act, (int)split);
     else
-        hipLaunchKernelGGL((k_slope_rows<T>), dim3((unsigned)((n + 63) / 64 * BIAS_SPLIT)), dim3(256), 0, st, (const T*)dy, (const T*)z,
-                           (T*)dz, partial, outer, n, act);
+        hipLaunchKernelGGL((k_slope_rows<T>), dim3((unsigned)(columns * split)), dim3(256), 0, st, (const T*)dy, (const T*)z,
+                           (T*)dz, partial, outer, n, act, (int)split);
     if (dbias)
-        hipLaunchKernelGGL((k_bias_join<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)dbias, n);
+        hipLaunchKernelGGL((k_bias_join<T>), dim3((unsigned)((n + 31) / 32)), dim3(256), 0, st, partial, (T*)dbias, n, (int)split);
     return dh_launch_status();
 }
 
