@@ -74,6 +74,17 @@ __global__ void __launch_bounds__(256) k_grad_power(const Table t, double* __res
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
         const int n = t.n[k] - at < CHUNK ? (int)(t.n[k] - at) : CHUNK;
+        if (n == CHUNK) {               // all of a full chunk's pieces are requested at once
+            constexpr int N = CHUNK / (256 * V);
+            T v[N][V];
+#pragma unroll
+            for (int u = 0; u < N; ++u) __builtin_memcpy(v[u], g + (u * 256 + threadIdx.x) * V, 16);
+#pragma unroll
+            for (int u = 0; u < N; ++u)
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum = join<KIND>(sum, power<KIND>(up(v[u][e])));
+            continue;
+        }
         for (int i = threadIdx.x * V; i < n; i += 256 * V) {
             T v[V];
             if (i + V <= n) __builtin_memcpy(v, g + i, 16);
@@ -128,6 +139,20 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* 
         const T* g = (const T*)t.in[k] + at;
         U* o = (U*)t.out[k] + at;
         const int n = t.n[k] - at < CHUNK ? (int)(t.n[k] - at) : CHUNK;
+        if (n == CHUNK) {
+            constexpr int N = CHUNK / (256 * V);
+            T v[N][V];
+#pragma unroll
+            for (int u = 0; u < N; ++u) __builtin_memcpy(v[u], g + (u * 256 + threadIdx.x) * V, 16);
+#pragma unroll
+            for (int u = 0; u < N; ++u) {
+                U w[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) w[e] = (U)(up(v[u][e]) * f);
+                __builtin_memcpy(o + (u * 256 + threadIdx.x) * V, w, sizeof(w));
+            }
+            continue;
+        }
         for (int i = threadIdx.x * V; i < n; i += 256 * V) {
             T v[V];
             U w[V];

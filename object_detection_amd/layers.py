@@ -153,8 +153,17 @@ class _Products(torch.autograd.Function):
         return tuple(outs)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
+        # grad mode is on only under create_graph: then the results are marked as having no further derivative
+        return (_Products._marked if torch.is_grad_enabled() else _Products._gradients)(ctx, *grads)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def _marked(ctx, *grads):
+        return _Products._gradients(ctx, *grads)
+
+    @staticmethod
+    def _gradients(ctx, *grads):
         rows, saved, wants = ctx.rows, ctx.saved_tensors, ctx.needs_input_grad
         result, inputs, weights, alive = [None, None], [], [], []
         for k, dy in enumerate(grads):
@@ -172,10 +181,10 @@ class _Products(torch.autograd.Function):
                 dz, db = (dy, torch.empty(n, dtype=dy.dtype, device=dy.device) if want_b else None) if at_weight else \
                     _slope(dy, z, ctx.act, want_b, outer, n, inner)
                 if want_x:
-                    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+                    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
                     inputs.append(_grad_input(rows, dz, w, dx))
                 if want_w:
-                    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+                    dw = torch.empty_like(w)
                     weights.append(_grad_weight(rows, dz, x, 0 if rows else _as_planes(x)[1], dw, db if at_weight else None))
                 alive.append(dz)
             result += [dx, dw, db, dy if want_r else None]
