@@ -22,6 +22,10 @@ typedef short s8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
+typedef unsigned int u2 __attribute__((ext_vector_type(2)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
 // ---- element types: conversions, and how many elements one 16-byte chunk holds ----
 template <typename T> struct Elem;
@@ -259,6 +263,7 @@ template <int N> __device__ __forceinline__ void wait_and_meet()
 // Feed (any alignment): through registers, one step ahead.
 template <typename T, int X, int BR, bool RC, bool PAIR, int THREADS>
 struct Feed {
+    typedef T type;
     typedef Tile<T, X, BR, RC, PAIR> TL;
     static constexpr int CH = Elem<T>::CH, N = TL::CHUNKS / THREADS, ROWS = THREADS / TL::ROW_CHUNKS;
     static_assert(TL::CHUNKS % THREADS == 0 && THREADS % TL::ROW_CHUNKS == 0, "whole rows of chunks per thread");
@@ -603,39 +608,17 @@ __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
-// Any alignment: one buffer in LDS behind DEPTH steps on their way in registers.
-template <typename T, int BI, int BJ, int BR, int WI, int WJ, int DEPTH, bool ARC, bool BRC>
-__global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
+// The reduction of one tile for operands of any alignment: one buffer in LDS behind DEPTH steps on their way in registers.
+// `put` brings a step's registers to LDS, `take` multiplies what is there.
+template <typename FA, typename FB, int BR, int DEPTH, typename Put, typename Take>
+__device__ __forceinline__ void pass_over(const Plan& q, const Place& at, Put&& put, Take&& take)
 {
-    constexpr int THREADS = WI * WJ * 64;
-    constexpr int TI = BI / WI / 16, TJ = BJ / WJ / 16;
-    typedef Feed<T, BI, BR, ARC, false, THREADS> FA;
-    typedef Feed<T, BJ, BR, BRC, sizeof(T) == 2, THREADS> FB;
-    typedef typename FA::TL TA;
-    typedef typename FB::TL TB;
-    __shared__ __align__(16) T lds[(BI + BJ) * BR];
-    T *lds_a = lds, *lds_b = lds + BI * BR;
-
-    Place at;
-    if (!place(L, BI, BJ, &at)) return;
-    const Plan& q = L.plan[at.w];
     const dh_product& p = q.p;
+    typedef typename FA::type T;
     const int k_begin = at.s * q.per, k_end = k_begin + q.per < q.steps ? k_begin + q.per : q.steps;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
     FA feed_a;
     FB feed_b;
     u4 ra[DEPTH][FA::N], rb[DEPTH][FB::N];
-    f4 acc[TI][TJ];
-#pragma unroll
-    for (int a = 0; a < TI; ++a)
-#pragma unroll
-        for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
-    f4 rows[TI];
-#pragma unroll
-    for (int a = 0; a < TI; ++a) rows[a] = f4{0.f, 0.f, 0.f, 0.f};
-    const bool sums = p.a_sum && at.j0 + wj == 0;
-
     int left = 0, batch = at.batch;
     auto enter = [&](int r0) {
         feed_a.begin((const T*)p.a + (int64_t)batch * p.a_batch, p.lda, at.i0, p.I, r0, p.R);
@@ -667,17 +650,178 @@ __global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
         for (int d = 0; d < DEPTH; ++d) {
             if (k + d >= k_end) break;
             __syncthreads();
-            FA::stage(lds_a, ra[d]);
-            FB::stage(lds_b, rb[d]);
+            put(ra[d], rb[d]);
             __syncthreads();
             if (k + d + DEPTH < k_end) fetch(d);
-            multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, lds_a, lds_b, wi, wj, lane);
+            take();
         }
     }
+}
+
+template <int TI, int TJ> __device__ __forceinline__ void clear(f4 (&acc)[TI][TJ], f4 (&rows)[TI])
+{
+#pragma unroll
+    for (int a = 0; a < TI; ++a) {
+        rows[a] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+
+template <typename T, int BI, int BJ, int BR, int WI, int WJ, int DEPTH, bool ARC, bool BRC>
+__global__ void __launch_bounds__(WI * WJ * 64) k_product_any(const Launch L)
+{
+    constexpr int THREADS = WI * WJ * 64;
+    constexpr int TI = BI / WI / 16, TJ = BJ / WJ / 16;
+    typedef Feed<T, BI, BR, ARC, false, THREADS> FA;
+    typedef Feed<T, BJ, BR, BRC, sizeof(T) == 2, THREADS> FB;
+    typedef typename FA::TL TA;
+    typedef typename FB::TL TB;
+    __shared__ __align__(16) T lds[(BI + BJ) * BR];
+    T *lds_a = lds, *lds_b = lds + BI * BR;
+
+    Place at;
+    if (!place(L, BI, BJ, &at)) return;
+    const Plan& q = L.plan[at.w];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    f4 acc[TI][TJ], rows[TI];
+    clear(acc, rows);
+    const bool sums = q.p.a_sum && at.j0 + wj == 0;
+    pass_over<FA, FB, BR, DEPTH>(
+        q, at, [&](const u4* ra, const u4* rb) { FA::stage(lds_a, ra); FB::stage(lds_b, rb); },
+        [&]() { multiply<T, TA, TB, BR, TI, TJ>(acc, rows, sums, lds_a, lds_b, wi, wj, lane); });
     static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
     __syncthreads();
     if (sums) row_sums<T, TI>(rows, q, at, at.i0 + wi);
     epilogue<T, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
+}
+
+// fp32 on the bf16 matrix instructions, whose rate is 16 times that of the fp32 ones: every value is split into three bf16 parts
+// (x = hi + mid + lo to 2^-25 of x: each part holds the next 8 bits, rounded), and of the nine products of parts the six are
+// formed that reach 2^-24 of the whole (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi; the three left out are below 2^-23 together).
+// A product of parts is exact in fp32 and sums are fp32, so this rounds where the fp32 instructions round.  What it cannot do is
+// found out and done again with those: a part of an infinity or NaN, or of a value that rounds to an infinity in bf16, leaves a
+// sum that is not finite; a part of a value below 2^-100 may underflow, which is looked for when the values are split.
+// Six products at 1/16 of the cost each: at best 2.7 times the fp32 rate; the split costs 7 vector instructions per value and
+// tile, which other workgroups' products hide.
+struct Split {
+    u2 hi, mid, lo;         // four values' parts
+};
+__device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
+{
+    Split s;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const f2 x = {__uint_as_float(v[2 * h]), __uint_as_float(v[2 * h + 1])};
+        const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, b2));
+        const f2 r = {x[0] - __uint_as_float(hi << 16), x[1] - __uint_as_float(hi & 0xFFFF0000u)};
+        const uint32_t mid = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, b2));
+        const f2 t = {r[0] - __uint_as_float(mid << 16), r[1] - __uint_as_float(mid & 0xFFFF0000u)};
+        s.hi[h] = hi;
+        s.mid[h] = mid;
+        s.lo[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, b2));
+        // the smallest magnitude but zero, per half: 0 - 1 is the largest 16-bit value
+        const us2 m = __builtin_bit_cast(us2, hi & 0x7FFF7FFFu) - us2{1, 1};
+        *smallest = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2, *smallest), m));
+    }
+    return s;
+}
+
+template <int BI, int BJ, int WI, int WJ, int DEPTH, int WAVES, bool ARC, bool BRC>
+__global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product_split(const Launch L)
+{
+    constexpr int THREADS = WI * WJ * 64, BR = 32;
+    constexpr int TI = BI / WI / 16, TJ = BJ / WJ / 16;
+    typedef Feed<float, BI, BR, ARC, false, THREADS> FA;
+    typedef Feed<float, BJ, BR, BRC, false, THREADS> FB;
+    typedef Tile<__bf16, BI, BR, ARC, false> TA;
+    typedef Tile<__bf16, BJ, BR, BRC, false> TB;
+    __shared__ __align__(16) __bf16 lds[3 * (BI + BJ) * BR];       // hi, mid, lo of A, then of B
+    __bf16 *la = lds, *lb = lds + 3 * BI * BR;
+
+    Place at;
+    if (!place(L, BI, BJ, &at)) return;
+    const Plan& q = L.plan[at.w];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = (wave / WJ) * (BI / WI), wj = (wave % WJ) * (BJ / WJ);
+    f4 acc[TI][TJ], rows[TI];
+    clear(acc, rows);
+    const bool sums = q.p.a_sum && at.j0 + wj == 0;
+    uint32_t smallest = 0xFFFFFFFFu;
+    auto put_one = [&](auto tile, __bf16* to, int plane, int k, u4 v) {
+        typedef decltype(tile) TL;
+        constexpr int ROW = TL::ROW_CHUNKS * 2;                     // 4-value pieces in a row
+        const int row = k / ROW, c = k % ROW;
+        __bf16* o = to + (row * TL::ROW_CHUNKS + ((c >> 1) ^ TL::key(row))) * 8 + (c & 1) * 4;
+        const Split s = split(v, &smallest);
+        *reinterpret_cast<u2*>(o) = s.hi;
+        *reinterpret_cast<u2*>(o + plane) = s.mid;
+        *reinterpret_cast<u2*>(o + 2 * plane) = s.lo;
+    };
+    pass_over<FA, FB, BR, DEPTH>(
+        q, at,
+        [&](const u4* ra, const u4* rb) {
+#pragma unroll
+            for (int k = 0; k < FA::N; ++k) put_one(TA(), la, BI * BR, k * THREADS + threadIdx.x, ra[k]);
+#pragma unroll
+            for (int k = 0; k < FB::N; ++k) put_one(TB(), lb, BJ * BR, k * THREADS + threadIdx.x, rb[k]);
+        },
+        [&]() {
+            s8 fb[TJ][3], ones;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ones[e] = 0x3F80;
+#pragma unroll
+            for (int b = 0; b < TJ; ++b)
+#pragma unroll
+                for (int h = 0; h < 3; ++h) fb[b][h] = TB::frag16(lb + h * BJ * BR, wj, b, 0, lane);
+#pragma unroll
+            for (int a = 0; a < TI; ++a) {
+                s8 fa[3];
+#pragma unroll
+                for (int h = 0; h < 3; ++h) fa[h] = TA::frag16(la + h * BI * BR, wi, a, 0, lane);
+                // the small products first
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][2], fa[0], acc[a][b]);
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][0], fa[2], acc[a][b]);
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][1], fa[1], acc[a][b]);
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][1], fa[0], acc[a][b]);
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][0], fa[1], acc[a][b]);
+#pragma unroll
+                for (int b = 0; b < TJ; ++b) acc[a][b] = mma16<__bf16>(fb[b][0], fa[0], acc[a][b]);
+                if (sums) {
+#pragma unroll
+                    for (int h = 2; h >= 0; --h) rows[a] = mma16<__bf16>(ones, fa[h], rows[a]);
+                }
+            }
+        });
+    // 2^-100 in bf16 is 0x0D80
+    bool again = (smallest & 0xFFFFu) < 0x0D7Fu || (smallest >> 16) < 0x0D7Fu;
+#pragma unroll
+    for (int a = 0; a < TI; ++a) {
+#pragma unroll
+        for (int b = 0; b < TJ; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) again |= !(fabsf(acc[a][b][e]) <= 3.402823466e38f);
+        again |= !(fabsf(rows[a][0]) <= 3.402823466e38f);
+    }
+    if (__syncthreads_or(again)) {
+        typedef typename FA::TL NA;
+        typedef typename FB::TL NB;
+        float *na = (float*)lds, *nb = na + BI * BR;
+        clear(acc, rows);
+        pass_over<FA, FB, BR, 1>(
+            q, at, [&](const u4* ra, const u4* rb) { FA::stage(na, ra); FB::stage(nb, rb); },
+            [&]() { multiply<float, NA, NB, BR, TI, TJ>(acc, rows, sums, na, nb, wi, wj, lane); });
+        __syncthreads();
+    }
+    static_assert(WI * WJ * TJ * 1024 <= (int)sizeof(lds), "room for the epilogue");
+    if (sums) row_sums<float, TI>(rows, q, at, at.i0 + wi);
+    epilogue<float, TB, TI, TJ>(acc, q, L.act, at, at.i0 + wi, at.j0 + wj, (float*)lds + wave * TJ * 256);
 }
 
 // One value of C through the epilogue.
@@ -849,6 +993,7 @@ __global__ void __launch_bounds__(256) k_product_join(const Launch L, const Join
 }
 
 constexpr int CUS = 256;
+constexpr int SPLIT = -1;              // stages of a shape whose fp32 values are split
 struct Shape { int bi, bj, br, stages; };        // br: bytes of a reduction step's row; bi = 0: the thin kernel
 
 // Tiles (i, j), bytes of a reduction step, waves along i and j, stages of the ring, waves per SIMD
@@ -884,7 +1029,9 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
     const dh_product& p = ps[0];
     if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
         return Shape{0, 16, 128, 1};
-    if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, 2};
+    const bool split = dtype == DH_F32 && shortest >= 64;
+    if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, split ? SPLIT : 2};
+    if (split) return Shape{128, 128, 128, SPLIT};
     if (!aligned) return Shape{128, 128, 128, 1};
     if (dtype != DH_F32 && huge >= 2 * CUS && shortest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
     return longest >= 1024 || large < CUS ? Shape{128, 128, 128, 2} : Shape{128, 128, 64, 3};
@@ -977,7 +1124,7 @@ void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
         }
         return;
     }
-    if (aligned) {
+    if (aligned && t.stages != SPLIT) {
 #define DH_CASE(BI, BJ, BYTES, WI, WJ, STAGES, WAVES) \
         if (t.bi == BI && t.bj == BJ && t.br == BYTES && t.stages == STAGES) { \
             hipLaunchKernelGGL((k_product<T, BI, BJ, BYTES / (int)sizeof(T), WI, WJ, STAGES, WAVES, ARC, BRC>), grid, dim3(WI * WJ * 64), 0, \
@@ -990,6 +1137,13 @@ void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
         }
 #undef DH_CASE
         return;
+    }
+    if constexpr (sizeof(T) == 4) {
+        if (t.stages == SPLIT) {
+            if (t.bi == 128) hipLaunchKernelGGL((k_product_split<128, 128, 2, 2, 1, 2, ARC, BRC>), grid, dim3(256), 0, st, L);
+            else hipLaunchKernelGGL((k_product_split<64, 64, 2, 2, 2, 3, ARC, BRC>), grid, dim3(256), 0, st, L);
+            return;
+        }
     }
     if (t.bi == 128) hipLaunchKernelGGL((k_product_any<T, 128, 128, BR, 2, 2, 1, ARC, BRC>), grid, dim3(256), 0, st, L);
     else hipLaunchKernelGGL((k_product_any<T, 64, 64, BR, 2, 2, 2, ARC, BRC>), grid, dim3(256), 0, st, L);

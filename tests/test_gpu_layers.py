@@ -278,6 +278,26 @@ def test_infinities_and_nan_stay_in_their_rows():
         close(y[rest], (want[0][rest], want[1][rest]), f"rest {dtype}")
 
 
+@pytest.mark.parametrize("small,large", [(1e-36, 1e6), (1e-30, 1e-6), (3e38, 1e-20), (2.0 ** -100, 1.0), (0.0, 1.0)])
+@pytest.mark.parametrize("size", [(70, 200, 90), (600, 96, 9000)])
+def test_fp32_over_its_whole_range(size, small, large):
+    """fp32 products of values near both ends of the range keep fp32's accuracy (their parts may leave bf16's, see the kernel)."""
+    from object_detection_amd.layers import linear
+    m, k, n = size
+    g = torch.Generator().manual_seed(9)
+    x = ((torch.rand((m, k), generator=g) + 0.1) / 1.1).mul_(small).cuda()
+    w = ((torch.rand((n, k), generator=g) - 0.5)).mul_(large).cuda()
+    with torch.no_grad():
+        y = linear(x, w)
+    close(y, rows64(x, w, None, None, None)["y"], "y")
+    mixed = x.clone()
+    mixed[:, ::3] = 0.0
+    mixed[5, 7] = 1e-38                     # one subnormal-to-be among ordinary values and zeros
+    with torch.no_grad():
+        y = linear(mixed, w)
+    close(y, rows64(mixed, w, None, None, None)["y"], "with zeros")
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
 def test_activations_far_out(act):
     """Pre-activations from -1e4 to 1e4: no overflow on the way, the limits of the functions at the ends."""
