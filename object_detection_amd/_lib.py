@@ -178,6 +178,23 @@ def lib():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The torch side of layers.py and grads.py (csrc/host.cpp), over the same library; like lib(), it never falls back."""
+    global _host
+    if _host is None:
+        lib()
+        try:
+            from . import _host as module
+        except ImportError as e:
+            raise ImportError("object_detection_amd/_host.so is missing or was built for another torch: build it with "
+                              "`make -C object_detection_amd/csrc`. There is no fallback path.") from e
+        _host = module
+    return _host
+
+
 def check(rc, name):
     if rc != 0:
         raise RuntimeError(f"{name} failed: {ERRORS.get(rc, rc)}")

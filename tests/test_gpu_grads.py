@@ -190,6 +190,7 @@ def test_refusals():
                  lambda: clip_grads([g], 1.0, out=[]), lambda: clip_grads([g], 1.0, out=[torch.ones(5, device="cuda")]),
                  lambda: clip_grads([g], 1.0, out=[g.half()]), lambda: clip_grads([g], 1.0, scale=torch.ones(2, device="cuda")),
                  lambda: clip_grads([g, g], 1.0, out=[g, g]), lambda: clip_grads([g, g + 1], 1.0, out=[g.clone(), g]),
+                 lambda: clip_grads([g, g], 1.0, out=[g, g.clone()]), lambda: clip_grads([g, g], 1.0, out=[g.clone(), g]),
                  lambda: total_grad_norm([g.to_sparse()]), lambda: total_grad_norm([torch.ones(3)])):
         with pytest.raises(RuntimeError):
             call()
