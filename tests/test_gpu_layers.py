@@ -126,7 +126,7 @@ def test_maps_channels_last(dtype):
 # reductions of each), with edges that fill no tile; the 64-bit side runs on the GPU.
 LARGE = [(4100, 136, 1040, "silu", True), (4100, 1048, 1040, "gelu", False), (8200, 520, 4080, None, True), (16, 4096, 2056, "silu", True),
          (17, 2056, 2100, "gelu", True), (32, 520, 4096, None, False), (5, 1001, 2049, "silu", True), (700, 8192, 72, "silu", True),
-         (3001, 333, 1501, "silu", True)]
+         (3001, 333, 1501, "silu", True), (1000, 333, 1001, "silu", True), (333, 1001, 1000, None, False), (700, 100, 900, "gelu", True)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
