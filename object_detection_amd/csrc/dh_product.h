@@ -109,15 +109,17 @@ struct Plan {               // one problem of a launch and how it is cut
     int batch_steps;        // reduction steps of one batch
     int split, per;         // workgroups along the reduction, and steps of each
     int out_batches;        // batches of the output (1 when the batch is reduced)
-    int first, count;       // first workgroup of this problem (a multiple of 8), and how many it has
+    int count;              // workgroups of this problem
+    dh_fastdiv by_plane, by_group, by_tail, by_batches;      // tiles_i tiles_j, 8 tiles_j, the last group's height, out_batches
     int stream;             // out and z are stored past the caches, in 16-byte pieces
     float* partial;         // split > 1: [split][out_batches][I][J]
     float* partial_sum;     // split > 1 and a_sum: [split][I]
 };
 
 struct Launch {
-    Plan plan[DH_MAX_PRODUCTS];
     int n, total, act;
+    int first[DH_MAX_PRODUCTS];     // first workgroup of each problem (a multiple of 8)
+    Plan plan[DH_MAX_PRODUCTS];
 };
 
 // An operand's tile in LDS.  X: rows of the tile along the operand's own index, BR: along the reduction.
@@ -388,22 +390,22 @@ struct Place {
 __device__ __forceinline__ bool place(const Launch& L, int BI, int BJ, Place* at)
 {
     int w = 0;
-    while (w + 1 < L.n && (int)blockIdx.x >= L.plan[w + 1].first) ++w;
+#pragma unroll
+    for (int k = 1; k < DH_MAX_PRODUCTS; ++k) w = k < L.n && (int)blockIdx.x >= L.first[k] ? k : w;
     const Plan& q = L.plan[w];
-    const int local = (int)blockIdx.x - q.first, per = (q.count + 7) / 8;       // q.first is a multiple of 8
-    int tile = (local & 7) * per + (local >> 3);
-    if ((local >> 3) >= per || tile >= q.count) return false;
-    const int plane = q.tiles_i * q.tiles_j;
-    const int rest = tile / plane;
+    const uint32_t local = blockIdx.x - L.first[w], per = (q.count + 7) / 8;
+    uint32_t tile = (local & 7) * per + (local >> 3);
+    if ((local >> 3) >= per || tile >= (uint32_t)q.count) return false;
+    const uint32_t plane = q.tiles_i * q.tiles_j, rest = dh_div(tile, q.by_plane);
     tile -= rest * plane;
-    const int group = tile / (8 * q.tiles_j), in = tile - group * 8 * q.tiles_j;
-    const int height = q.tiles_i - group * 8 < 8 ? q.tiles_i - group * 8 : 8;
-    const int tj = in / height;
+    const uint32_t group = dh_div(tile, q.by_group), in = tile - group * 8 * q.tiles_j;
+    const uint32_t height = q.tiles_i - group * 8;
+    const uint32_t tj = height >= 8 ? in >> 3 : dh_div(in, q.by_tail);
     at->w = w;
-    at->i0 = (group * 8 + in - tj * height) * BI;
-    at->j0 = tj * BJ;
-    at->s = rest / q.out_batches;
-    at->batch = rest - at->s * q.out_batches;
+    at->i0 = (int)(group * 8 + in - tj * (height >= 8 ? 8 : height)) * BI;
+    at->j0 = (int)tj * BJ;
+    at->s = (int)dh_div(rest, q.by_batches);
+    at->batch = (int)rest - at->s * q.out_batches;
     return true;
 }
 

@@ -42,6 +42,8 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
     return longest >= 1024 || large < CUS ? Shape{128, 128, 128, 2} : Shape{128, 128, 64, 3};
 }
 
+uint32_t at_least_1(int v) { return v > 0 ? (uint32_t)v : 1u; }
+
 int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws_bytes, bool* aligned, Shape* shape)
 {
     const int64_t ch = dtype == DH_F32 ? 4 : 8, size = dtype == DH_F32 ? 4 : 2;
@@ -109,8 +111,12 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
             q.partial_sum = (float*)((char*)ws + bytes);
             if (p.a_sum) bytes += ((size_t)q.split * p.I * sizeof(float) + 255) & ~(size_t)255;
         }
-        q.first = (int)total;
+        L->first[w] = (int)total;
         q.count = (int)(tiles * q.split);
+        q.by_plane = dh_make_fastdiv(at_least_1(q.tiles_i * q.tiles_j));
+        q.by_group = dh_make_fastdiv(at_least_1(8 * q.tiles_j));
+        q.by_tail = dh_make_fastdiv(at_least_1(q.tiles_i % 8));
+        q.by_batches = dh_make_fastdiv(at_least_1(q.out_batches));
         total += (tiles * q.split + 7) / 8 * 8;
         if (total >= (1ll << 30)) return DH_ERR_ARG;
     }
