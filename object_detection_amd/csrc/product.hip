@@ -73,9 +73,10 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     }
     // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
     // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each.
-    // Tiles for half of the CUs to all of them, without the ring of the aligned kernels: two groups of waves in one workgroup
-    // share a tile's reduction and join in LDS (1023 x 777 -> 1001 fp32: 24 us against 30 alone and 29 cut and joined by a launch).
-    const bool grouped = t.bi == 64 && all_tiles <= CUS && all_tiles >= CUS / 2 && (!*aligned || t.stages == SPLIT);
+    // Tiles for three quarters of the CUs to all of them, without the ring of the aligned kernels: two groups of waves in one workgroup
+    // share a tile's reduction and join in LDS (1023 x 777 -> 1001 fp32: 24 us against 30 alone and 29 cut and joined by a launch; but
+    // 128 x 4096 -> 4096, 128 tiles: 85 against 47).
+    const bool grouped = t.bi == 64 && all_tiles <= CUS && all_tiles >= CUS * 3 / 4 && (!*aligned || t.stages == SPLIT);
     if (grouped) shape->groups = 2;
     const bool cutting = t.bi && all_tiles < CUS && !grouped;
     int64_t each = (tile_steps + 2 * CUS - 1) / (2 * CUS);
