@@ -71,15 +71,19 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         all_tiles += tiles;
         tile_steps += tiles * ((p.R + br - 1) / br) * (p.reduce_batch ? p.batch : 1);
     }
-    // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
-    // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each.
     // Tiles for three quarters of the CUs to all of them, without the ring of the aligned kernels: two groups of waves in one workgroup
     // share a tile's reduction and join in LDS (1023 x 777 -> 1001 fp32: 24 us against 30 alone and 29 cut and joined by a launch; but
     // 128 x 4096 -> 4096, 128 tiles: 85 against 47).
     const bool grouped = t.bi == 64 && all_tiles <= CUS && all_tiles >= CUS * 3 / 4 && (!*aligned || t.stages == SPLIT);
     if (grouped) shape->groups = 2;
-    const bool cutting = t.bi && all_tiles < CUS && !grouped;
-    int64_t each = (tile_steps + 2 * CUS - 1) / (2 * CUS);
+    // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
+    // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each (1024^3 bf16, 256
+    // tiles of 64 x 64, uncut: 11 us against 17).  About as many tiles as CUs are cut too where the reduction is long: one workgroup of a
+    // CU has nothing beside it while it waits (4096 x 1024 over 8192 rows, 256 tiles of 128 x 128: bf16 78 us against 102, fp32 377
+    // against 544).
+    const int64_t once = 2 * CUS;
+    int64_t each = (tile_steps + once - 1) / once;
+    const bool cutting = t.bi && !grouped && (all_tiles < CUS || (t.bi == 128 && all_tiles <= CUS * 5 / 4 && each >= 4096 / t.br));
     if (each < 1024 / t.br) each = 1024 / t.br;
     int order[DH_MAX_PRODUCTS];
     for (int w = 0; w < n; ++w) {          // long reductions first: their workgroups are the ones a launch waits for
