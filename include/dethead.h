@@ -540,6 +540,7 @@ int dh_regression_loss_bwd(const float* pred, const float* target, const float* 
  * pointers and strides are faster.  workspace: 16-byte aligned, dh_products_workspace() bytes (may be 0); the same products
  * captured into two graphs that run at once need two of them. */
 #define DH_MAX_PRODUCTS 5
+#define DH_MAX_EXTENT 2147482623      /* of i, j and r: 2^31 - 1025 */
 enum { DH_F32 = 0, DH_F16 = 1, DH_BF16 = 2 };
 enum { DH_ACT_NONE = 0, DH_ACT_RELU = 1, DH_ACT_SILU = 2, DH_ACT_GELU = 3, DH_ACT_SIGMOID = 4, DH_ACT_LAST = 4 };
 typedef struct dh_product {

@@ -253,7 +253,7 @@ struct Stream {
 
     __device__ void one(uint32_t to, uint32_t from) const
     {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(from), "s"(base) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(from), "s"(base) : "m0", "memory");
     }
 };
 

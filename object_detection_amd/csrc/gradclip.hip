@@ -179,8 +179,8 @@ int64_t chunks_of(const int64_t* n, int lo, int hi)
     return c;
 }
 
-// the table of tensors lo..hi-1; false if it holds more chunks than an int counts
-bool fill(Table* t, const void* const* in, void* const* out, const int64_t* n, int lo, int hi, int* chunks)
+// the table of tensors lo..hi-1 and how many chunks it has (sized() has bounded them)
+int fill(Table* t, const void* const* in, void* const* out, const int64_t* n, int lo, int hi)
 {
     int64_t c = 0;
     for (int k = lo; k < hi; ++k) {
@@ -189,19 +189,21 @@ bool fill(Table* t, const void* const* in, void* const* out, const int64_t* n, i
         t->n[k - lo] = n[k];
         t->first[k - lo] = (int)c;
         c += (n[k] + CHUNK - 1) / CHUNK;
-        if (c >= (1ll << 31)) return false;
     }
     t->count = hi - lo;
     t->first[hi - lo] = (int)c;
-    *chunks = (int)c;
-    return true;
+    return (int)c;
 }
 
 bool sized(const int64_t* n, int count)
 {
     if (count < 0 || (count > 0 && !n)) return false;
-    for (int k = 0; k < count; ++k)
+    int64_t chunks = 0;                     // chunk numbers and their strides stay within an int
+    for (int k = 0; k < count; ++k) {
         if (n[k] < 0 || n[k] >= (1ll << 40)) return false;
+        chunks += (n[k] + CHUNK - 1) / CHUNK;
+        if (chunks >= (1ll << 30)) return false;
+    }
     return true;
 }
 
@@ -260,8 +262,7 @@ extern "C" int dh_grad_power(const void* const* grads, const int64_t* n, int cou
     hipStream_t st = (hipStream_t)stream;
     for (int lo = 0; lo < count; lo += TABLE) {
         Table t;
-        int chunks = 0;
-        if (!fill(&t, grads, nullptr, n, lo, lo + TABLE < count ? lo + TABLE : count, &chunks)) return DH_ERR_ARG;
+        const int chunks = fill(&t, grads, nullptr, n, lo, lo + TABLE < count ? lo + TABLE : count);
         if (chunks == 0) continue;
         const int groups = groups_of(chunks);
         if (dtype == DH_F32) launch_power<float>(t, norm, groups, partial, st);
@@ -296,8 +297,7 @@ extern "C" int dh_grad_clip(const void* const* grads, void* const* out, const in
     bool told = false;
     for (int lo = 0; lo < count; lo += TABLE) {
         Table t;
-        int chunks = 0;
-        if (!fill(&t, grads, out, n, lo, lo + TABLE < count ? lo + TABLE : count, &chunks)) return DH_ERR_ARG;
+        const int chunks = fill(&t, grads, out, n, lo, lo + TABLE < count ? lo + TABLE : count);
         if (chunks == 0) continue;
         const int groups = groups_of(chunks);
         float* say = told ? nullptr : norm_out;

@@ -78,7 +78,7 @@ void check_tensors(const char* where, Item& it)
     if (at::autocast::is_autocast_enabled(at::kCUDA)) {
         const at::ScalarType to = at::autocast::get_autocast_dtype(at::kCUDA);
         for (Tensor* t : it.all())
-            if (t->defined() && t->is_floating_point() && t->scalar_type() != to) *t = t->to(to);
+            if (t->defined() && t->is_floating_point() && t->scalar_type() != at::kDouble && t->scalar_type() != to) *t = t->to(to);
     }
     const at::ScalarType type = it.x.scalar_type();
     for (Tensor* t : it.all())
@@ -116,7 +116,7 @@ Tensor as_planes(const Tensor& t)
 
 int as_int(int64_t v)
 {
-    if (v < 0 || v > INT32_MAX) fail("a dimension of a product exceeds 2^31 - 1");
+    if (v < 0 || v > DH_MAX_EXTENT) fail("a dimension of a product exceeds " + std::to_string(DH_MAX_EXTENT));
     return (int)v;
 }
 

@@ -139,6 +139,8 @@ int check(const dh_product* ps, int n, int dtype, int activation)
     for (int w = 0; w < n; ++w) {
         const dh_product& p = ps[w];
         if (p.I < 0 || p.J < 0 || p.R < 0 || p.batch < 0 || p.lda < 0 || p.ldb < 0 || p.ldo < 0 || p.ldr < 0) return DH_ERR_ARG;
+        if (p.a_batch < 0 || p.b_batch < 0 || p.o_batch < 0 || p.res_batch < 0) return DH_ERR_ARG;
+        if (p.I > DH_MAX_EXTENT || p.J > DH_MAX_EXTENT || p.R > DH_MAX_EXTENT) return DH_ERR_ARG;      // the last tile's end is an int
         if (!!p.a_by_reduction != !!ps[0].a_by_reduction || !!p.b_by_reduction != !!ps[0].b_by_reduction) return DH_ERR_ARG;
         if (!p.a_by_reduction && p.b_by_reduction) return DH_ERR_ARG;      // no caller has that pair
         const bool work = p.I > 0 && p.J > 0 && (p.reduce_batch || p.batch > 0);
@@ -195,6 +197,7 @@ extern "C" int dh_product_slope(const void* dy, const void* z, void* dz, void* d
     if (outer * inner > 0 && (!dy || (z && !dz))) return DH_ERR_ARG;
     if (dbias && (!workspace || workspace_bytes < dh_product_slope_workspace(n))) return DH_ERR_WORKSPACE;
     if (dbias && !dh_aligned16(workspace)) return DH_ERR_ALIGN;
+    if (((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)dbias) % (dtype == DH_F32 ? 4 : 2)) return DH_ERR_ALIGN;
     hipStream_t st = (hipStream_t)stream;
     float* ws = (float*)workspace;
     if (dtype == DH_F32) return launch_slope<float>(dy, z, dz, dbias, outer, n, inner, activation, ws, st);

@@ -400,8 +400,8 @@ class Detect(nn.Module):
         return grid, anchor_grid
 
     def _convolutions(self, x):
-        """yolo.py:52 for every level."""
-        if self.fused_convs and all(type(m) is nn.Conv2d for m in self.m):
+        """yolo.py:52 for every level.  On the CPU (the pass that derives the strides) and for replaced layers, the layers themselves."""
+        if self.fused_convs and all(v.is_cuda for v in x[:self.nl]) and all(type(m) is nn.Conv2d for m in self.m):
             return head_convs(x[:self.nl], [m.weight for m in self.m], [m.bias for m in self.m])
         return [self.m[i](x[i]) for i in range(self.nl)]
 

@@ -340,6 +340,46 @@ def test_gradient_against_differences():
         assert (got - slope).abs() < bound, (act, float(got), float(slope), float(bound))
 
 
+@pytest.mark.parametrize("which", [0, 1, 2, 3, (0, 3), (1, 2), (2, 3)])
+@pytest.mark.parametrize("act", [None, "silu"])
+def test_gradients_of_some_inputs_only(which, act):
+    """Each of x, weight, bias and residual alone, and pairs of them: the wanted gradients and no others."""
+    from object_detection_amd.layers import head_convs, linear
+    which = which if isinstance(which, tuple) else (which,)
+    x, w, b, r, dy = rows_case(33, 40, 24, torch.float32, act, True, True)
+    want = rows64(x, w, b, act, r, dy)
+    t = [v.cuda().requires_grad_(k in which) for k, v in enumerate((x, w, b, r))]
+    linear(t[0], t[1], t[2], act, t[3]).backward(dy.cuda())
+    for k, name in enumerate(("dx", "dw", "db", "dr")):
+        if k in which:
+            close(t[k].grad, want[name], name)
+        else:
+            assert t[k].grad is None
+    # levels without a bias between levels with one, only some of them trained
+    xs = [x.view(1, 33, 40, 1).permute(0, 2, 1, 3).cuda() for _ in range(3)]
+    ws, bs = [w.cuda().requires_grad_(l != 1) for l in range(3)], [b.cuda().requires_grad_(True), None, b.cuda().requires_grad_(True)]
+    ys = head_convs(xs, ws, bs)
+    (ys[0].sum() + 2 * ys[2].sum()).backward()          # level 1 takes no part
+    one = rows64(x, w, b, None, None, torch.ones(33, 24))
+    two = rows64(x, w, b, None, None, torch.full((33, 24), 2.0))
+    close(ws[0].grad, one["dw"], "level 0")
+    close(ws[2].grad, two["dw"], "level 2")
+    close(bs[0].grad, one["db"], "level 0 bias")
+    close(bs[2].grad, two["db"], "level 2 bias")
+    assert ws[1].grad is None
+
+
+def test_saved_inputs_are_guarded():
+    """An input that is overwritten between forward and backward is an error, not a wrong gradient."""
+    from object_detection_amd.layers import linear
+    x, w, _, _, _ = rows_case(8, 16, 8, torch.float32, None, False, False)
+    gx, gw = x.cuda(), w.cuda().requires_grad_(True)
+    y = linear(gx, gw)
+    gx.zero_()
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
 def test_autocast_casts_like_torch_layers():
     from object_detection_amd.layers import head_convs, linear
     x, w, b, _, _ = rows_case(9, 32, 24, torch.float32, None, True, False)
@@ -439,7 +479,7 @@ def test_refuses_what_it_cannot_do():
                  lambda: pointwise_conv(x, w), lambda: pointwise_conv(x.view(1, 8, 2, 2), torch.zeros(6, 8, 3, 3, device="cuda")),
                  lambda: pointwise_conv(x.view(1, 8, 2, 2), w, residual=torch.zeros(1, 6, 2, 3, device="cuda")),
                  lambda: head_convs([], [], []), lambda: head_convs([x.view(1, 8, 2, 2)] * 6, [w] * 6, [None] * 6),
-                 lambda: head_convs([x.view(1, 8, 2, 2)], [w, w], [None]),
+                 lambda: head_convs([x.view(1, 8, 2, 2)], [w, w], [None]), lambda: linear(x.to_sparse(), w), lambda: linear(x.long(), w.long()),
                  lambda: head_convs([x.view(1, 8, 2, 2), x.half().view(1, 8, 2, 2)], [w, w.half()], [None, None])):
         with pytest.raises(RuntimeError):
             call()

@@ -53,6 +53,9 @@ def test_entry_refuses_bad_arguments():
     assert call(I=-1) == -1 and call(J=-1) == -1 and call(R=-1) == -1 and call(batch=-1) == -1
     assert call(lda=-1) == -1 and call(ldo=-4) == -1
     assert call(a_by_reduction=0) == -1
+    assert call(a_batch=-1) == -1 and call(res_batch=-8) == -1
+    assert call(I=(1 << 31) - 1) == -1 and call(R=(1 << 31) - 512) == -1
+    assert call(a_sum=4096, batch=2) == -1 and call(a_sum=4096, J=0) == -1
     assert call(a=4098) == -3 and call(dtype=1, out=16385) == -3
     assert call(R=1 << 16, lda=1 << 16, ldb=1 << 16) == -4                      # a split reduction needs its workspace
     assert call(I=1 << 30, J=1 << 30) == -1                                     # more tiles than a launch has
@@ -62,3 +65,13 @@ def test_entry_refuses_bad_arguments():
     assert lib.dh_product_slope(4096, 4096, None, None, 8, 8, 8, 2, 0, None, 0, None) == -1
     assert lib.dh_product_slope(4096, None, None, 4096, 8, 8, 8, 0, 0, None, 0, None) == -4
     assert lib.dh_product_slope(4096, None, None, 4096, 8, 8, 8, 9, 0, None, 0, None) == -1
+    assert lib.dh_product_slope(4098, None, None, 4096, 8, 8, 8, 0, 0, 8192, 1 << 20, None) == -3
+
+
+def test_detect_with_fused_convolutions_on_the_cpu():
+    """The pass on the CPU that derives a model's strides goes through the layers themselves."""
+    from object_detection_amd.yolo import Detect
+    det = Detect(3, [[1, 2, 3, 4]], (4,))
+    det.fused_convs = True
+    det.train()
+    assert det([torch.zeros(1, 4, 5, 6)])[0].shape == (1, 2, 5, 6, 8)
