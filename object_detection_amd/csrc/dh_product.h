@@ -274,7 +274,8 @@ struct Feed {
     const T* last;          // the last address from which a whole chunk can be read
     int64_t step;
     bool live;              // C: this thread's columns exist
-    bool inside;            // the whole tile exists
+    bool inside;            // the whole tile can be read
+    int beyond;             // C at an edge: elements that one further row certainly has, up to a chunk
 
     __device__ static int tid() { return threadIdx.x & (THREADS - 1); }      // in the group of THREADS that shares a tile
 
@@ -287,11 +288,16 @@ struct Feed {
                 const int x = x0 + row + k * ROWS;
                 at[k] = base + (int64_t)(x < xend ? x : xend - 1) * ld + r0 + c * CH;      // rows behind the end: never stored
             } else {
-                at[k] = base + (int64_t)(r0 + row + k * ROWS) * ld + x0 + c * CH;
+                // columns behind the end repeat the last ones: never stored
+                const int x = x0 + c * CH < xend || xend < CH ? x0 + c * CH : xend - CH;
+                at[k] = base + (int64_t)(r0 + row + k * ROWS) * ld + x;
             }
         }
         live = RC || x0 + c * CH < xend;
-        inside = x0 + X <= xend;
+        // R: rows are clamped, so only the reduction can end.  C: a chunk over the end of a row reads on into the next one (columns
+        // that are not stored), as long as 16 bytes of rows follow this step
+        inside = RC || x0 + X <= xend;
+        beyond = xend < CH ? 0 : (ld < CH ? (int)ld : CH);
         step = RC ? BR : BR * ld;
         last = base + (RC ? (int64_t)(xend - 1) * ld + rend : (int64_t)(rend - 1) * ld + xend) - CH;
     }
@@ -299,7 +305,8 @@ struct Feed {
     // the chunks of a step of which `left` reduction values remain (BR or more: all); what lies behind them becomes zero
     __device__ void fetch(u4* v, int left)
     {
-        if (inside && left >= BR) {
+        const int after = left - BR < CH ? left - BR : CH;
+        if (left >= BR && (inside || after * beyond >= CH)) {
 #pragma unroll
             for (int k = 0; k < N; ++k) __builtin_memcpy(&v[k], at[k], 16);
         } else {
