@@ -14,8 +14,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
-#include <unordered_map>
-#include <unordered_set>
+#include <utility>
 #include <vector>
 
 namespace py = pybind11;
@@ -503,12 +502,43 @@ Tensor total_norm(const variable_list& grads, int norm, const py::object& scale,
     return out;
 }
 
+// Two workgroups must not scale one tensor, nor read what another writes: no tensor is written twice, and one that is written is
+// read as its own gradient only.
+void apart(const char* where, const variable_list& read, const variable_list& written, bool in_place)
+{
+    typedef std::pair<const void*, size_t> At;
+    const auto sorted = [](const variable_list& tensors) {
+        std::vector<At> v;
+        v.reserve(tensors.size());
+        for (size_t k = 0; k < tensors.size(); ++k)
+            if (tensors[k].numel()) v.emplace_back(tensors[k].data_ptr(), k);
+        std::sort(v.begin(), v.end());
+        return v;
+    };
+    const std::vector<At> to = sorted(written);
+    for (size_t k = 1; k < to.size(); ++k)
+        if (to[k].first == to[k - 1].first) fail(std::string(where) + ": a gradient is in the list twice");
+    if (in_place) return;                   // read where it is written
+    const std::vector<At> from = sorted(read);
+    for (size_t r = 0, w = 0; r < from.size() && w < to.size();) {
+        if (from[r].first < to[w].first) ++r;
+        else if (to[w].first < from[r].first) ++w;
+        else {
+            if (r + 1 < from.size() && from[r + 1].first == from[r].first) fail(std::string(where) + ": a gradient is in the list twice");
+            if (from[r].second != to[w].second) fail(std::string(where) + ": an output is another gradient of the list");
+            ++r;
+        }
+    }
+}
+
 // Norm, and outs[k] = grads[k] / scale * factor; without outs in place.
 Tensor clip(const char* where, const variable_list& grads, const std::optional<variable_list>& outs, double limit, int norm,
             const py::object& scale, const py::object& reduce)
 {
     const at::NoGradGuard off;
     variable_list read, written;
+    read.reserve(grads.size());
+    written.reserve(grads.size());
     const std::vector<List> lists = listed(where, grads, &read);
     const variable_list& into = outs ? *outs : grads;
     if (into.size() != grads.size())
@@ -532,14 +562,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
         std::vector<void*> to;
     };
     std::vector<Out> launches;
-    std::unordered_map<const void*, size_t> where_read;
-    std::unordered_set<const void*> seen;
-    constexpr size_t many = (size_t)-1;
-    for (size_t k = 0; k < read.size(); ++k)
-        if (read[k].numel()) {
-            const auto put = where_read.emplace(read[k].data_ptr(), k);
-            if (!put.second) put.first->second = many;
-        }
+    apart(where, read, written, !outs);
     for (const List& l : lists)
         for (const at::ScalarType type : {l.type, at::kFloat}) {
             if (type == l.type && !launches.empty() && launches.back().list.type == l.type && launches.back().type == type) continue;
@@ -547,17 +570,9 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
             for (size_t e = 0; e < l.index.size(); ++e) {
                 const size_t k = l.index[e];
                 if (written[k].scalar_type() != type) continue;
-                void* to = written[k].data_ptr();
-                if (l.n[e]) {
-                    // two workgroups must not scale one tensor, nor read what another writes
-                    const auto hit = where_read.find(to);
-                    if (!seen.insert(to).second || (hit != where_read.end() && hit->second == many))
-                        fail(std::string(where) + ": a gradient is in the list twice");
-                    if (hit != where_read.end() && hit->second != k) fail(std::string(where) + ": an output is another gradient of the list");
-                }
                 o.list.at.push_back(l.at[e]);
                 o.list.n.push_back(l.n[e]);
-                o.to.push_back(to);
+                o.to.push_back(written[k].data_ptr());
             }
             if (!o.to.empty()) launches.push_back(std::move(o));
         }
