@@ -546,7 +546,11 @@ __device__ __forceinline__ void epilogue(f4 (&acc)[TI][TJ], const Plan& q, int a
     }
 }
 
-// Aligned operands: a ring of STAGES buffers in LDS, the copies of STAGES - 1 steps on their way while one is multiplied.
+// Aligned operands: a ring of STAGES buffers in LDS, the copies of STAGES - 1 steps on their way while one is multiplied (copied by
+// the memory system itself, so that a step costs no registers and one barrier).
+// Large reductions are bound by the matrix pipes: 8192^3 bf16 1357 TFLOP/s; with 1024 to reduce the prologue and the epilogue of
+// a tile show, 8192 x 1024 -> 4096 bf16 69 us = 999 TFLOP/s, with gelu 80 (862).  Maps with few channels are bound by bytes: 128 ->
+// 128 channels, silu and residual of 64 x 80 x 80 cells (315 MB) 75 us = 4.2 TB/s, where a plain copy of that card reaches 4.9.
 template <typename T, int BI, int BJ, int BR, int WI, int WJ, int STAGES, int WAVES, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
 {
@@ -711,6 +715,10 @@ __device__ __forceinline__ void join_groups(f4 (&acc)[TI][TJ], f4 (&rows)[TI], i
     __syncthreads();
 }
 
+// Operands that the copies above cannot take (rows of a number of bytes that is no multiple of 16, unaligned pointers) and fp32 with
+// less than 64 to reduce.  Bound by the instructions that bring a step to LDS: each 16 bytes pass through registers, with a shift
+// where their row is not aligned.  8191 x 1023 -> 4095 bf16 134 us = 512 TFLOP/s, half of what the aligned neighbour reaches; 1023 x 777
+// -> 1001 bf16 11.9 us, of which a 64 x 64 tile's 13 steps, one after another, are the most.
 // GROUPS > 1: tiles that fill the chip only once are worked on by that many groups of waves, which share the reduction.
 template <typename T, int BI, int BJ, int BR, int WI, int WJ, int DEPTH, int GROUPS, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS) k_product_any(const Launch L)
@@ -779,6 +787,10 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
     return s;
 }
 
+// fp32 products, six bf16 ones each (above).  Long reductions are bound by the vector instructions that split beside the matrix
+// instructions that multiply: 8192 x 1024 -> 4096 353 us = 195 TFLOP/s, 8192^3 198, where the card's fp32 matrix instructions end at
+// 157.  The head's levels at batch 64 (733 MB of 916 written) take 404 us: 266 of memory and 283 of products, which overlap between
+// the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
 template <int BI, int BJ, int WI, int WJ, int DEPTH, int WAVES, int GROUPS, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(const Launch L)
 {
@@ -896,6 +908,7 @@ template <typename T> __device__ __forceinline__ void finish_one(const dh_produc
 // waves take the reduction in turns of 128 bytes, fragments come from memory straight into registers (no row is used twice, so
 // LDS would only add a trip), and the waves' sums are added in order at the end.  Lane (m, g) reads 32 consecutive bytes of row
 // m, for two products of which each pairs the same reduction values of A and B; which values those are does not matter.
+// One token, 4096 -> 16384 bf16: 24 us = 5.5 TB/s of weight; 4096 -> 4096 7.1 us = 4.7 TB/s (and 16 tokens 9.4).
 template <typename T, int MI>
 __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
 {
@@ -983,7 +996,8 @@ __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
 
 // Sums the partial products of the workgroups along the reduction, in a fixed order, and finishes them.  A thread adds four
 // values' parts, eight requested at a time; with many parts, eight threads share them (every eighth part each) and their sums are
-// added in turn.  All products of a launch that were split join in one launch.
+// added in turn.  All products of a launch that were split join in one launch.  Bound by the trip to memory: 17 MB of parts, the
+// head's weight gradients at batch 64, 12 us beside 101 for their products.
 struct Joins {
     int w[DH_MAX_PRODUCTS], first[DH_MAX_PRODUCTS + 1], n;
     int share[DH_MAX_PRODUCTS];             // 1 or 8 threads per value

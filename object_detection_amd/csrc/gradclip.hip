@@ -5,6 +5,10 @@
 // of the gradients: the factor needs the norm of all of them, so they are read twice.  Sums are doubles from the first element
 // on: a square of an fp32 gradient may leave fp32's range, and a sum over 10^8 elements needs more than 24 bits.  No atomics:
 // the result does not depend on the order in which workgroups run.
+//
+// 2^29 elements in 64 tensors: the norm 6.1 TB/s (fp32 351 us, bf16 175), the norm and the scaled copy 5.4 and 5.2 TB/s over the
+// three passes (1185 and 617 us).  Below about 30 MB the launches and the host's walk over the list are longer than the bytes:
+// 31 chunks of a head's gradients 11 us, 111 tensors of 7 M fp16 values 23 us, of which the two kernels are 19.
 #include "../../include/dethead.h"
 #include "dh_common.h"
 
