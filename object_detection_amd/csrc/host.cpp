@@ -66,11 +66,16 @@ struct Item {
     std::array<Tensor*, 4> all() { return {&x, &w, &bias, &res}; }
 };
 
+// The kernels read memory: a view whose sign is kept beside it (the imaginary part of a conjugate) is written out first.
+Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // One supported type on one ROCm device; under autocast its type.
 void check_tensors(const char* where, Item& it)
 {
     if (!it.x.is_cuda())
         fail(std::string(where) + ": x is on " + it.x.device().str() + ": object_detection_amd only runs on ROCm devices (no CPU fallback)");
+    for (Tensor* t : it.all())
+        if (t->defined() && t->is_neg()) *t = t->resolve_neg();
     for (Tensor* t : it.all())
         if (t->defined() && t->device() != it.x.device())
             fail(std::string(where) + ": tensors on " + t->device().str() + " and " + it.x.device().str());
@@ -311,7 +316,7 @@ struct Products : torch::autograd::Function<Products> {
             if (!grads[k].defined()) continue;
             const Tensor &x = saved[3 * k], &w = saved[3 * k + 1], &z = saved[3 * k + 2];
             const bool want_x = wanted(4 * k), want_w = wanted(4 * k + 1), want_b = wanted(4 * k + 2), want_r = wanted(4 * k + 3);
-            const Tensor dy = grads[k].contiguous();
+            const Tensor dy = in_memory(grads[k]).contiguous();
             Tensor* to = &result[2 + 4 * k];
             if (want_r) to[3] = dy;
             if (!want_x && !want_w && !want_b) continue;
@@ -447,7 +452,7 @@ std::vector<List> listed(const char* where, const variable_list& grads, variable
             lists.push_back({type, {}, {}, {}, 0});
             it = lists.end() - 1;
         }
-        const Tensor r = dense(g) ? g : g.contiguous();
+        const Tensor r = in_memory(dense(g) ? g : g.contiguous());
         it->at.push_back(r.data_ptr());
         it->n.push_back(r.numel());
         it->index.push_back(k);
@@ -551,7 +556,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
                      (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)))
             fail(std::string(where) + ": an output must have its gradient's number of elements and device, and its type or fp32");
         // elements in one piece and in the order they are read in, or through a copy
-        const bool direct = (read[k].is_contiguous() && o.is_contiguous()) || (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides());
+        const bool direct = !o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) || (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides()));
         written.push_back(direct ? o : at::empty_like(read[k], read[k].options().dtype(o.scalar_type())));
         copies |= !direct;
     }

@@ -204,6 +204,22 @@ def test_refusals():
     assert torch.equal(q.grad, g)
 
 
+def test_views_with_the_sign_beside_them():
+    """The imaginary part of a conjugate is a view of the memory of its negative."""
+    from object_detection_amd.grads import clip_grad_norm_, clip_grads
+    c = torch.tensor([[3.0 + 4.0j]], device="cuda")
+    g = c.conj().imag
+    assert g.is_neg() and float(g) == -4.0
+    norm, (out,) = clip_grads([g], 2.0)
+    assert float(norm) == 4.0
+    torch.testing.assert_close(out.cpu(), torch.full((1, 1), -2.0), rtol=1e-6, atol=0)      # (2 / (4 + 1e-6) is 2.5e-7 off)
+    q = torch.nn.Parameter(torch.zeros(1, 1, device="cuda"))
+    q.grad = g
+    clip_grad_norm_([q], 2.0)
+    torch.testing.assert_close(q.grad.cpu(), torch.full((1, 1), -2.0), rtol=1e-6, atol=0)
+    torch.testing.assert_close(c.cpu().imag, torch.full((1, 1), 2.0), rtol=1e-6, atol=0)
+
+
 def test_streams_and_graph_replay():
     from object_detection_amd.grads import clip_grads
     grads = made(SHAPES, torch.float16, 6)

@@ -489,3 +489,19 @@ def test_refuses_what_it_cannot_do():
     g, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+def test_views_with_the_sign_beside_them():
+    """The imaginary part of a conjugate is a view of the memory of its negative: as input, weight, bias, residual and gradient."""
+    from object_detection_amd.layers import linear
+    c = torch.tensor([[2.0 + 3.0j]], device="cuda")
+    v = c.conj().imag
+    assert v.is_neg() and float(v) == -3.0
+    one, two = torch.ones(1, 1, device="cuda"), torch.full((1, 1), 2.0, device="cuda")
+    assert float(linear(v, two)) == -6.0
+    assert float(linear(two, v)) == -6.0
+    assert float(linear(two, one, v[0], None, v)) == -4.0
+    x = two.clone().requires_grad_(True)
+    y = linear(x, two)
+    (dx,) = torch.autograd.grad(y, x, v)
+    assert float(dx) == -6.0
