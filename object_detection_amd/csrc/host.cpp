@@ -507,32 +507,39 @@ Tensor total_norm(const variable_list& grads, int norm, const py::object& scale,
     return out;
 }
 
-// Two workgroups must not scale one tensor, nor read what another writes: no tensor is written twice, and one that is written is
-// read as its own gradient only.
+// Two workgroups must not scale one piece of memory, nor read what another writes: nothing is written twice, and what is written
+// is read by its own gradient only, at the same places.
 void apart(const char* where, const variable_list& read, const variable_list& written, bool in_place)
 {
-    typedef std::pair<const void*, size_t> At;
+    struct At {
+        const char *begin, *end;
+        size_t k;
+        bool operator<(const At& o) const { return begin < o.begin; }
+    };
     const auto sorted = [](const variable_list& tensors) {
         std::vector<At> v;
         v.reserve(tensors.size());
         for (size_t k = 0; k < tensors.size(); ++k)
-            if (tensors[k].numel()) v.emplace_back(tensors[k].data_ptr(), k);
+            if (tensors[k].numel()) {
+                const char* at = (const char*)tensors[k].data_ptr();
+                v.push_back({at, at + tensors[k].nbytes(), k});
+            }
         std::sort(v.begin(), v.end());
         return v;
     };
     const std::vector<At> to = sorted(written);
     for (size_t k = 1; k < to.size(); ++k)
-        if (to[k].first == to[k - 1].first) fail(std::string(where) + ": a gradient is in the list twice");
+        if (to[k].begin < to[k - 1].end) fail(std::string(where) + ": a gradient is in the list twice, or two outputs overlap");
     if (in_place) return;                   // read where it is written
+    // what is read is in the order of its beginnings, what is written is apart: the outputs behind every gradient that begins
+    // later than they end are left behind, and each gradient is held against those it reaches
     const std::vector<At> from = sorted(read);
-    for (size_t r = 0, w = 0; r < from.size() && w < to.size();) {
-        if (from[r].first < to[w].first) ++r;
-        else if (to[w].first < from[r].first) ++w;
-        else {
-            if (r + 1 < from.size() && from[r + 1].first == from[r].first) fail(std::string(where) + ": a gradient is in the list twice");
-            if (from[r].second != to[w].second) fail(std::string(where) + ": an output is another gradient of the list");
-            ++r;
-        }
+    size_t w = 0;
+    for (const At& r : from) {
+        while (w < to.size() && to[w].end <= r.begin) ++w;
+        for (size_t o = w; o < to.size() && to[o].begin < r.end; ++o)
+            if (to[o].k != r.k || to[o].begin != r.begin || to[o].end != r.end)
+                fail(std::string(where) + ": an output overlaps a gradient of the list that is not its own");
     }
 }
 

@@ -204,6 +204,24 @@ def test_refusals():
     assert torch.equal(q.grad, g)
 
 
+def test_overlapping_outputs_are_refused():
+    from object_detection_amd.grads import clip_grads
+    flat = torch.arange(24, device="cuda", dtype=torch.float32)
+    kept, half = flat.clone(), torch.ones(16, device="cuda", dtype=torch.float16)
+    a, b = torch.ones(8, device="cuda"), torch.ones(8, device="cuda")
+    for grads, out in (([a, b], [flat[0:8], flat[7:15]]),               # two outputs share an element
+                       ([flat[0:8], b], [a.clone(), flat[4:12]]),       # an output inside another's gradient
+                       ([flat[0:24], b], [torch.zeros(24, device="cuda"), flat[16:24]]),
+                       ([flat[0:8]], [flat[1:9]]),                      # an output shifted against its own gradient
+                       ([half[0:8]], [half.view(torch.float32)])):      # fp32 written over the fp16 that is read
+        with pytest.raises(RuntimeError, match="overlap"):
+            clip_grads(grads, 1.0, out=out)
+    assert torch.equal(flat, kept)
+    # neighbours are apart, and one may be written in place while the next is not
+    norm, _ = clip_grads([flat[0:8], flat[8:16]], 1e9, out=[flat[0:8], flat[16:24]])
+    assert torch.equal(flat[16:24], kept[8:16]) and torch.equal(flat[0:16], kept[0:16])
+
+
 def test_views_with_the_sign_beside_them():
     """The imaginary part of a conjugate is a view of the memory of its negative."""
     from object_detection_amd.grads import clip_grad_norm_, clip_grads
