@@ -73,7 +73,12 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     no synchronisation.  scale, group: as in total_grad_norm() (with a scale the gradients come out unscaled)."""
     code, limit = _norm_code("clip_grad_norm_", norm_type), _limit("clip_grad_norm_", max_norm)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    parameters = list(parameters)
     grads = [g for g in [p.grad for p in parameters] if g is not None]
+    if not grads and group is not None:         # this rank has nothing to add, the others wait for it all the same
+        if not parameters:
+            raise RuntimeError("clip_grad_norm_: a rank of a group needs at least one parameter")
+        grads = [parameters[0].detach().new_empty(0)]
     if not grads:
         return torch.zeros(())
     if error_if_nonfinite:

@@ -204,6 +204,22 @@ def test_refusals():
     assert torch.equal(q.grad, g)
 
 
+def test_a_rank_without_gradients_takes_part_in_the_exchange(monkeypatch):
+    from object_detection_amd import grads as G
+    met = []
+
+    def exchange(power, norm_type, group):
+        met.append((float(power), norm_type, group))
+        return power + 16.0                     # what the other ranks hold
+    monkeypatch.setattr(G, "all_reduce_norm_power", exchange)
+    p = torch.nn.Parameter(torch.zeros(3, device="cuda"))
+    assert float(G.clip_grad_norm_([p], 1.0, group=True)) == 4.0 and met == [(0.0, 2.0, None)]
+    assert p.grad is None
+    with pytest.raises(RuntimeError, match="at least one parameter"):
+        G.clip_grad_norm_([], 1.0, group=True)
+    assert float(G.clip_grad_norm_([p], 1.0)) == 0.0 and len(met) == 1
+
+
 def test_overlapping_outputs_are_refused():
     from object_detection_amd.grads import clip_grads
     flat = torch.arange(24, device="cuda", dtype=torch.float32)
