@@ -344,6 +344,12 @@ def clip_augmented(y, nl):
     return y
 
 
+def _plain_conv(m):
+    """A 1x1 convolution whose call is its product and nothing else."""
+    return (type(m) is nn.Conv2d and m.kernel_size == (1, 1) and m.stride == (1, 1) and m.padding == (0, 0) and m.groups == 1
+            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks))
+
+
 class Detect(nn.Module):
     """Same constructor, buffers and forward contract as yolo.py:33-70.
 
@@ -400,8 +406,9 @@ class Detect(nn.Module):
         return grid, anchor_grid
 
     def _convolutions(self, x):
-        """yolo.py:52 for every level.  On the CPU (the pass that derives the strides) and for replaced layers, the layers themselves."""
-        if self.fused_convs and all(v.is_cuda for v in x[:self.nl]) and all(type(m) is nn.Conv2d for m in self.m):
+        """yolo.py:52 for every level.  On the CPU (the pass that derives the strides), for replaced layers and for layers with hooks
+        (pruning and the like rebuild the weight in one), the layers themselves."""
+        if self.fused_convs and all(v.is_cuda for v in x[:self.nl]) and all(_plain_conv(m) for m in self.m):
             return head_convs(x[:self.nl], [m.weight for m in self.m], [m.bias for m in self.m])
         return [self.m[i](x[i]) for i in range(self.nl)]
 

@@ -75,3 +75,18 @@ def test_detect_with_fused_convolutions_on_the_cpu():
     det.fused_convs = True
     det.train()
     assert det([torch.zeros(1, 4, 5, 6)])[0].shape == (1, 2, 5, 6, 8)
+
+
+def test_which_layers_the_fused_head_replaces():
+    from object_detection_amd.yolo import _plain_conv
+    nn = torch.nn
+    assert _plain_conv(nn.Conv2d(4, 6, 1)) and _plain_conv(nn.Conv2d(4, 6, 1, bias=False))
+    for m in (nn.Conv2d(4, 6, 3), nn.Conv2d(4, 6, 1, stride=2), nn.Conv2d(4, 6, 1, padding=1), nn.Conv2d(4, 6, 1, groups=2),
+              nn.Sequential(nn.Conv2d(4, 6, 1))):
+        assert not _plain_conv(m)
+    for hook in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook", "register_full_backward_pre_hook"):
+        m = nn.Conv2d(4, 6, 1)
+        handle = getattr(m, hook)(lambda *a: None)
+        assert not _plain_conv(m)
+        handle.remove()
+        assert _plain_conv(m)
