@@ -194,7 +194,9 @@ extern "C" int dh_product_slope(const void* dy, const void* z, void* dz, void* d
     if (outer < 0 || n < 0 || inner < 0 || dtype < DH_F32 || dtype > DH_BF16 || activation < 0 || activation > DH_ACT_LAST) return DH_ERR_ARG;
     if (n == 0 || (!z && !dbias)) return DH_OK;
     if (n >= (1ll << 24) || outer >= (1ll << 40) || inner >= (1ll << 40)) return DH_ERR_ARG;
-    if (outer * inner > 0 && (!dy || (z && !dz))) return DH_ERR_ARG;
+    int64_t per, all;
+    if (__builtin_mul_overflow(outer, inner, &per) || __builtin_mul_overflow(per, n, &all) || all >= (1ll << 60)) return DH_ERR_ARG;
+    if (per > 0 && (!dy || (z && !dz))) return DH_ERR_ARG;
     if (dbias && (!workspace || workspace_bytes < dh_product_slope_workspace(n))) return DH_ERR_WORKSPACE;
     if (dbias && !dh_aligned16(workspace)) return DH_ERR_ALIGN;
     if (((uintptr_t)dy | (uintptr_t)z | (uintptr_t)dz | (uintptr_t)dbias) % (dtype == DH_F32 ? 4 : 2)) return DH_ERR_ALIGN;

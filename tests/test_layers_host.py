@@ -90,3 +90,11 @@ def test_which_layers_the_fused_head_replaces():
         assert not _plain_conv(m)
         handle.remove()
         assert _plain_conv(m)
+
+
+def test_slope_entry_refuses_extents_whose_product_leaves_64_bits():
+    from object_detection_amd import _lib as L
+    far = 1 << 39
+    for z in (None, 4096):
+        assert L.lib().dh_product_slope(None, z, None, 4096, far, 1 << 20, far, 2, 0, 8192, 1 << 40, None) == -1
+    assert L.lib().dh_product_slope(None, None, None, 4096, far, 1 << 23, 1, 0, 0, 8192, 1 << 40, None) == -1
