@@ -135,10 +135,12 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* 
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n_all;
     double factor = max_norm / (n_all + 1e-6);
     factor = factor > 1.0 ? 1.0 : factor;               // (a NaN norm leaves a NaN factor)
-    const float f = (float)(factor / by);
+    // as two floats: a factor near the end of fp32's range (norms of 1e38 do not leave it) would lose its bits in one
+    const double both = factor / by;
+    const float f2 = both < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(f2 == 1.f ? both : both * 0x1p64);
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const int k = find(t, c);
-        if (f == 1.0f && t.in[k] == t.out[k]) continue;   // in place and nothing to do
+        if (f == 1.f && f2 == 1.f && t.in[k] == t.out[k]) continue;   // in place and nothing to do
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
         U* o = (U*)t.out[k] + at;
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* 
             for (int u = 0; u < N; ++u) {
                 U w[V];
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = (U)(up(v[u][e]) * f);
+                for (int e = 0; e < V; ++e) w[e] = (U)(up(v[u][e]) * f * f2);
                 __builtin_memcpy(o + (u * 256 + threadIdx.x) * V, w, sizeof(w));
             }
             continue;
@@ -163,12 +165,12 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* 
             if (i + V <= n) {
                 __builtin_memcpy(v, g + i, 16);
 #pragma unroll
-                for (int e = 0; e < V; ++e) w[e] = (U)(up(v[e]) * f);
+                for (int e = 0; e < V; ++e) w[e] = (U)(up(v[e]) * f * f2);
                 __builtin_memcpy(o + i, w, sizeof(w));
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    if (i + e < n) o[i + e] = (U)(up(g[i + e]) * f);
+                    if (i + e < n) o[i + e] = (U)(up(g[i + e]) * f * f2);
             }
         }
     }

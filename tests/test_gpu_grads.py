@@ -220,6 +220,18 @@ def test_a_rank_without_gradients_takes_part_in_the_exchange(monkeypatch):
     assert float(G.clip_grad_norm_([p], 1.0)) == 0.0 and len(met) == 1
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_the_normal_range(dtype):
+    """Norms near the end of fp32's range against a small bound: the factor is below 2^-126, the results are not."""
+    from object_detection_amd.grads import clip_grads
+    g = (torch.randn(10000, generator=torch.Generator().manual_seed(11)) * 1e36).to(dtype)
+    norm, (out,) = clip_grads([g.cuda()], 1e-6, out=[torch.empty(10000, device="cuda")])
+    want = g.double() * (1e-6 / (g.double().norm() + 1e-6))
+    assert 1e-6 / float(norm) < 2.0 ** -140
+    # two roundings (the factor, the product) and the exact one by 2^-64: 2^-24 each, and 2^-150 where a result is subnormal
+    torch.testing.assert_close(out.cpu().double(), want, rtol=2.1 * 2.0 ** -24, atol=2.0 ** -149)
+
+
 def test_overlapping_outputs_are_refused():
     from object_detection_amd.grads import clip_grads
     flat = torch.arange(24, device="cuda", dtype=torch.float32)
