@@ -107,7 +107,13 @@ __global__ void __launch_bounds__(256) k_grad_power(const Table t, double* __res
 template <int KIND> __device__ __forceinline__ double total(const double* __restrict__ partial, int parts, double* shared)
 {
     double sum = 0.0;
-    for (int i = threadIdx.x; i < parts; i += 256) sum = join<KIND>(sum, partial[i]);
+    for (int i = threadIdx.x; i < parts; i += 256 * 8) {        // eight requested at once: a trip to L2 each is what this costs
+        double v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = i + 256 * u < parts ? partial[i + 256 * u] : 0.0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum = join<KIND>(sum, v[u]);
+    }
     return group_join<KIND>(sum, shared);
 }
 
