@@ -1,6 +1,6 @@
 // Norm of many gradients taken as one vector, and their scaling by min(1, max_norm / (norm + 1e-6)).
 //
-// Two launches per (up to) 120 tensors, whatever their sizes: the first sums |g|^p into one double per workgroup, the second
+// Two launches for (up to) 280 tensors, whatever their sizes (176 where the results go to other tensors): the first sums |g|^p into one double per workgroup, the second
 // adds those sums in their order -- every workgroup for itself, 8 KB that sit in L2 -- and scales.  Both are bound by the bytes
 // of the gradients: the factor needs the norm of all of them, so they are read twice.  Sums are doubles from the first element
 // on: a square of an fp32 gradient may leave fp32's range, and a sum over 10^8 elements needs more than 24 bits.  No atomics:
@@ -11,20 +11,28 @@
 // 31 chunks of a head's gradients 11 us, 111 tensors of 7 M fp16 values 23 us, of which the two kernels are 19.
 #include "../../include/dethead.h"
 #include "dh_common.h"
+#include <algorithm>
 
 namespace {
 
-constexpr int TABLE = 120;          // tensors of one launch: the table travels as a kernel argument (4 KB at most)
+constexpr int READ = 280, BOTH = 176;       // tensors of one launch: the table travels as a kernel argument (4 KB at most)
 constexpr int CHUNK = 8192;         // elements a workgroup takes at a time
 constexpr int GROUPS = 1024;        // workgroups of a launch at most: 4 per CU
 
-struct Table {
-    const void* in[TABLE];
-    void* out[TABLE];
-    int64_t n[TABLE];
-    int first[TABLE + 1];           // first chunk of each tensor
+// OUT: with other tensors for the results; without, what is read is what is written.
+template <bool OUT> struct Table {
+    static constexpr int SIZE = OUT ? BOTH : READ;
+    void* in[SIZE];
+    void* to[OUT ? SIZE : 1];
+    int first[SIZE + 1];            // first chunk of each tensor
+    uint16_t tail[SIZE];            // elements of each tensor's last chunk
     int count;
+
+    __device__ void* out(int k) const { return OUT ? to[k] : in[k]; }
+    __device__ int length(int k, int chunk) const { return chunk + 1 < first[k + 1] ? CHUNK : tail[k]; }
 };
+static_assert(sizeof(Table<true>) <= 4096 - 64 && sizeof(Table<false>) <= 4096 - 64, "beside the other arguments");
+static_assert(CHUNK < 65536, "a tail has 16 bits");
 
 template <typename T> __device__ __forceinline__ float up(T v) { return (float)v; }
 
@@ -56,7 +64,7 @@ template <int KIND> __device__ __forceinline__ double group_join(double v, doubl
     return join<KIND>(join<KIND>(shared[0], shared[1]), join<KIND>(shared[2], shared[3]));
 }
 
-__device__ __forceinline__ int find(const Table& t, int chunk)
+template <bool OUT> __device__ __forceinline__ int find(const Table<OUT>& t, int chunk)
 {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
@@ -68,7 +76,7 @@ __device__ __forceinline__ int find(const Table& t, int chunk)
 }
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(256) k_grad_power(const Table t, double* __restrict__ partial)
+__global__ void __launch_bounds__(256) k_grad_power(const Table<false> t, double* __restrict__ partial)
 {
     constexpr int V = 16 / sizeof(T);
     __shared__ double shared[4];
@@ -77,7 +85,7 @@ __global__ void __launch_bounds__(256) k_grad_power(const Table t, double* __res
         const int k = find(t, c);
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
-        const int n = t.n[k] - at < CHUNK ? (int)(t.n[k] - at) : CHUNK;
+        const int n = t.length(k, c);
         if (n == CHUNK) {               // all of a full chunk's pieces are requested at once
             constexpr int N = CHUNK / (256 * V);
             T v[N][V];
@@ -129,8 +137,8 @@ __global__ void __launch_bounds__(256) k_grad_join(const double* __restrict__ pa
     }
 }
 
-template <typename T, typename U, int KIND>
-__global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* __restrict__ partial, int parts,
+template <typename T, typename U, int KIND, bool OUT>
+__global__ void __launch_bounds__(256) k_grad_clip(const Table<OUT> t, const double* __restrict__ partial, int parts,
                                                    const float* __restrict__ scale, double max_norm, float* __restrict__ norm)
 {
     constexpr int V = 16 / sizeof(T);
@@ -146,11 +154,11 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table t, const double* 
     const float f2 = both < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(f2 == 1.f ? both : both * 0x1p64);
     for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
         const int k = find(t, c);
-        if (f == 1.f && f2 == 1.f && t.in[k] == t.out[k]) continue;   // in place and nothing to do
+        if (f == 1.f && f2 == 1.f && t.in[k] == t.out(k)) continue;   // in place and nothing to do
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
-        U* o = (U*)t.out[k] + at;
-        const int n = t.n[k] - at < CHUNK ? (int)(t.n[k] - at) : CHUNK;
+        U* o = (U*)t.out(k) + at;
+        const int n = t.length(k, c);
         if (n == CHUNK) {
             constexpr int N = CHUNK / (256 * V);
             T v[N][V];
@@ -191,15 +199,17 @@ int64_t chunks_of(const int64_t* n, int lo, int hi)
     return c;
 }
 
-// the table of tensors lo..hi-1 and how many chunks it has (sized() has bounded them)
-int fill(Table* t, const void* const* in, void* const* out, const int64_t* n, int lo, int hi)
+// the table of tensors lo.. and how many chunks it has (sized() has bounded them)
+template <bool OUT>
+int fill(Table<OUT>* t, const void* const* in, void* const* out, const int64_t* n, int lo, int count)
 {
+    const int hi = lo + t->SIZE < count ? lo + t->SIZE : count;
     int64_t c = 0;
     for (int k = lo; k < hi; ++k) {
-        t->in[k - lo] = in[k];
-        t->out[k - lo] = out ? out[k] : nullptr;
-        t->n[k - lo] = n[k];
+        t->in[k - lo] = (void*)in[k];
+        if (OUT) t->to[k - lo] = out[k];
         t->first[k - lo] = (int)c;
+        t->tail[k - lo] = (uint16_t)(n[k] ? (n[k] - 1) % CHUNK + 1 : 0);
         c += (n[k] + CHUNK - 1) / CHUNK;
     }
     t->count = hi - lo;
@@ -220,27 +230,51 @@ bool sized(const int64_t* n, int count)
 }
 
 template <typename T, int KIND>
-void launch_power(const Table& t, int groups, double* partial, hipStream_t st)
+void launch_power(const Table<false>& t, int groups, double* partial, hipStream_t st)
 {
     hipLaunchKernelGGL((k_grad_power<T, KIND>), dim3((unsigned)groups), dim3(256), 0, st, t, partial);
 }
 
 template <typename T>
-void launch_power(const Table& t, int kind, int groups, double* partial, hipStream_t st)
+void launch_power(const Table<false>& t, int kind, int groups, double* partial, hipStream_t st)
 {
     if (kind == DH_NORM_1) launch_power<T, DH_NORM_1>(t, groups, partial, st);
     else if (kind == DH_NORM_2) launch_power<T, DH_NORM_2>(t, groups, partial, st);
     else launch_power<T, DH_NORM_MAX>(t, groups, partial, st);
 }
 
-template <typename T, typename U>
-void launch_clip(const Table& t, int kind, int groups, const double* partial, int parts, const float* scale, double max_norm, float* norm,
+template <typename T, typename U, bool OUT>
+void launch_clip(const Table<OUT>& t, int kind, int groups, const double* partial, int parts, const float* scale, double max_norm, float* norm,
                  hipStream_t st)
 {
     const dim3 grid((unsigned)groups), block(256);
-    if (kind == DH_NORM_1) hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_1>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
-    else if (kind == DH_NORM_2) hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_2>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
-    else hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_MAX>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
+    if (kind == DH_NORM_1) hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_1, OUT>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
+    else if (kind == DH_NORM_2) hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_2, OUT>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
+    else hipLaunchKernelGGL((k_grad_clip<T, U, DH_NORM_MAX, OUT>), grid, block, 0, st, t, partial, parts, scale, max_norm, norm);
+}
+
+// All tensors of a list; whether there were any elements.  `norm` receives its value from the first launch.
+template <bool OUT>
+bool clip_all(const void* const* grads, void* const* out, const int64_t* n, int count, int dtype, int out_dtype, int kind, const double* partial,
+              int parts, const float* scale, double max_norm, float* norm, hipStream_t st)
+{
+    bool told = false;
+    for (int lo = 0; lo < count; lo += Table<OUT>::SIZE) {
+        Table<OUT> t;
+        const int chunks = fill(&t, grads, out, n, lo, count);
+        if (chunks == 0) continue;
+        const int groups = groups_of(chunks);
+        float* say = told ? nullptr : norm;
+        told = true;
+        if (dtype == DH_F32) launch_clip<float, float>(t, kind, groups, partial, parts, scale, max_norm, say, st);
+        else if (dtype == DH_F16 && out_dtype == DH_F16) launch_clip<_Float16, _Float16>(t, kind, groups, partial, parts, scale, max_norm, say, st);
+        else if (dtype == DH_BF16 && out_dtype == DH_BF16) launch_clip<__bf16, __bf16>(t, kind, groups, partial, parts, scale, max_norm, say, st);
+        else if constexpr (OUT) {
+            if (dtype == DH_F16) launch_clip<_Float16, float>(t, kind, groups, partial, parts, scale, max_norm, say, st);
+            else launch_clip<__bf16, float>(t, kind, groups, partial, parts, scale, max_norm, say, st);
+        }
+    }
+    return told;
 }
 
 bool types(int dtype) { return dtype >= DH_F32 && dtype <= DH_BF16; }
@@ -252,8 +286,8 @@ extern "C" int64_t dh_grad_parts(const int64_t* n, int count)
 {
     if (!sized(n, count)) return 0;
     int64_t parts = 0;
-    for (int lo = 0; lo < count; lo += TABLE) {
-        const int hi = lo + TABLE < count ? lo + TABLE : count;
+    for (int lo = 0; lo < count; lo += READ) {
+        const int hi = lo + READ < count ? lo + READ : count;
         const int64_t c = chunks_of(n, lo, hi);
         parts += c < GROUPS ? c : GROUPS;
     }
@@ -272,9 +306,9 @@ extern "C" int dh_grad_power(const void* const* grads, const int64_t* n, int cou
     if (parts < need) return DH_ERR_WORKSPACE;
     if (need && (!partial || (uintptr_t)partial % 8)) return DH_ERR_ARG;
     hipStream_t st = (hipStream_t)stream;
-    for (int lo = 0; lo < count; lo += TABLE) {
-        Table t;
-        const int chunks = fill(&t, grads, nullptr, n, lo, lo + TABLE < count ? lo + TABLE : count);
+    for (int lo = 0; lo < count; lo += READ) {
+        Table<false> t;
+        const int chunks = fill(&t, grads, nullptr, n, lo, count);
         if (chunks == 0) continue;
         const int groups = groups_of(chunks);
         if (dtype == DH_F32) launch_power<float>(t, norm, groups, partial, st);
@@ -306,20 +340,9 @@ extern "C" int dh_grad_clip(const void* const* grads, void* const* out, const in
         if ((uintptr_t)grads[k] % (dtype == DH_F32 ? 4 : 2) || (uintptr_t)out[k] % (out_dtype == DH_F32 ? 4 : 2)) return DH_ERR_ALIGN;
     }
     hipStream_t st = (hipStream_t)stream;
-    bool told = false;
-    for (int lo = 0; lo < count; lo += TABLE) {
-        Table t;
-        const int chunks = fill(&t, grads, out, n, lo, lo + TABLE < count ? lo + TABLE : count);
-        if (chunks == 0) continue;
-        const int groups = groups_of(chunks);
-        float* say = told ? nullptr : norm_out;
-        told = true;
-        if (dtype == DH_F32) launch_clip<float, float>(t, norm, groups, partial, (int)parts, scale, max_norm, say, st);
-        else if (dtype == DH_F16 && out_dtype == DH_F16) launch_clip<_Float16, _Float16>(t, norm, groups, partial, (int)parts, scale, max_norm, say, st);
-        else if (dtype == DH_F16) launch_clip<_Float16, float>(t, norm, groups, partial, (int)parts, scale, max_norm, say, st);
-        else if (out_dtype == DH_BF16) launch_clip<__bf16, __bf16>(t, norm, groups, partial, (int)parts, scale, max_norm, say, st);
-        else launch_clip<__bf16, float>(t, norm, groups, partial, (int)parts, scale, max_norm, say, st);
-    }
+    const bool in_place = out_dtype == dtype && std::equal(grads, grads + count, out);
+    const bool told = in_place ? clip_all<false>(grads, out, n, count, dtype, out_dtype, norm, partial, (int)parts, scale, max_norm, norm_out, st)
+                               : clip_all<true>(grads, out, n, count, dtype, out_dtype, norm, partial, (int)parts, scale, max_norm, norm_out, st);
     if (!told && norm_out) return dh_grad_norm(partial, parts, norm, scale, nullptr, norm_out, stream);      // nothing to scale
     return dh_launch_status();
 }

@@ -304,6 +304,32 @@ def test_large_list():
         assert float((o.double() - t.double() * f).abs().max()) <= float(t.abs().max()) * f * 3 * U32 * 1.001
 
 
+@pytest.mark.parametrize("count", [176, 177, 280, 281, 600])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lists_around_what_a_launch_takes(dtype, count):
+    """Tables that are just full, and several of them; empty tensors at their ends; whole and partial last chunks."""
+    from object_detection_amd.grads import clip_grads, total_grad_norm
+    sizes = [(0,) if k % 88 in (0, 87) else ((k * 977) % 9000 + 1,) if k % 7 else (8192 * (k % 3 + 1),) for k in range(count)]
+    grads = made(sizes, dtype, 12)
+    norm = norm64(grads, 2.0)
+    near(total_grad_norm(grads), norm)
+    for limit in (norm / 3, norm * 3):
+        n, out = clip_grads(grads, limit)
+        near(n, norm)
+        clipped_close(out, grads, norm, limit)
+        n, out = clip_grads(grads, limit, out=[torch.empty(s, device="cuda") for s in sizes])
+        near(n, norm)
+        clipped_close(out, grads, norm, limit)
+        mine = [g.clone() for g in grads]
+        n, _ = clip_grads(mine, limit, out=mine)
+        near(n, norm)
+        clipped_close(mine, grads, norm, limit)
+        half = [g.clone() for g in grads]                       # every other tensor in place
+        n, out = clip_grads(half, limit, out=[g if k % 2 else torch.empty_like(g) for k, g in enumerate(half)])
+        near(n, norm)
+        clipped_close(out, grads, norm, limit)
+
+
 def test_training_step_of_the_head():
     """Detect's convolutions, the loss on their outputs, the gradients back to the weights and their clipping, in one run: against
     torch's convolutions on the same device in fp32 and the clipping formula."""
