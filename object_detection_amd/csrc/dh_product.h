@@ -761,13 +761,15 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS) k_product_any(const Lau
 // formed that reach 2^-24 of the whole (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi; the three left out are below 2^-23 together).
 // A product of parts is exact in fp32 and sums are fp32, so this rounds where the fp32 instructions round.  What it cannot do is
 // found out and done again with those: a part of an infinity or NaN, or of a value that rounds to an infinity in bf16, leaves a
-// sum that is not finite; a part of a value below 2^-100 may underflow, which is looked for when the values are split.
+// sum that is not finite; a part of a value below 2^-100 may underflow, which is looked for when the values are split.  Such a value
+// is off by 2^-124 at most, its product by that times the other operand's largest: sums that reach 2^25 times what R of
+// those add up to need nothing (a few underflowing gradients among others; without this a tile that held one took twice as long).
 // Six products at 1/16 of the cost each: at best 2.7 times the fp32 rate; the split costs 7 vector instructions per value and
 // tile, which other workgroups' products hide.
 struct Split {
     u2 hi, mid, lo;         // four values' parts
 };
-__device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
+__device__ __forceinline__ Split split(u4 v, uint32_t* smallest, uint32_t* largest)
 {
     Split s;
 #pragma unroll
@@ -781,8 +783,9 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
         s.mid[h] = mid;
         s.lo[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, b2));
         // the smallest magnitude but zero, per half: 0 - 1 is the largest 16-bit value
-        const us2 m = __builtin_bit_cast(us2, hi & 0x7FFF7FFFu) - us2{1, 1};
+        const us2 size = __builtin_bit_cast(us2, hi & 0x7FFF7FFFu), m = size - us2{1, 1};
         *smallest = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2, *smallest), m));
+        *largest = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, *largest), size));
     }
     return s;
 }
@@ -791,6 +794,15 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
 // instructions that multiply: 8192 x 1024 -> 4096 353 us = 195 TFLOP/s, 8192^3 198, where the card's fp32 matrix instructions end at
 // 157.  The head's levels at batch 64 (733 MB of 916 written) take 404 us: 266 of memory and 283 of products, which overlap between
 // the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
+__device__ __forceinline__ float wave_most(uint32_t pair)        // above the magnitude of every value whose first parts made `pair`
+{
+    const uint32_t lo = pair & 0xFFFFu, hi = pair >> 16;
+    float v = __uint_as_float(((lo > hi ? lo : hi) + 1) << 16);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
 template <int BI, int BJ, int WI, int WJ, int DEPTH, int WAVES, int GROUPS, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(const Launch L)
 {
@@ -812,13 +824,13 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
     f4 acc[TI][TJ], rows[TI];
     clear(acc, rows);
     const bool sums = q.p.a_sum && at.j0 + wj == 0;
-    uint32_t smallest = 0xFFFFFFFFu;
-    auto put_one = [&](auto tile, __bf16* to, int plane, int k, u4 v) {
+    uint32_t smallest = 0xFFFFFFFFu, largest_a = 0, largest_b = 0;
+    auto put_one = [&](auto tile, __bf16* to, int plane, int k, u4 v, uint32_t* largest) {
         typedef decltype(tile) TL;
         constexpr int ROW = TL::ROW_CHUNKS * 2;                     // 4-value pieces in a row
         const int row = k / ROW, c = k % ROW;
         __bf16* o = to + (row * TL::ROW_CHUNKS + ((c >> 1) ^ TL::key(row))) * 8 + (c & 1) * 4;
-        const Split s = split(v, &smallest);
+        const Split s = split(v, &smallest, largest);
         *reinterpret_cast<u2*>(o) = s.hi;
         *reinterpret_cast<u2*>(o + plane) = s.mid;
         *reinterpret_cast<u2*>(o + 2 * plane) = s.lo;
@@ -827,9 +839,9 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
         q, at, group, GROUPS,
         [&](const u4* ra, const u4* rb) {
 #pragma unroll
-            for (int k = 0; k < FA::N; ++k) put_one(TA(), la, BI * BR, k * THREADS + tid, ra[k]);
+            for (int k = 0; k < FA::N; ++k) put_one(TA(), la, BI * BR, k * THREADS + tid, ra[k], &largest_a);
 #pragma unroll
-            for (int k = 0; k < FB::N; ++k) put_one(TB(), lb, BJ * BR, k * THREADS + tid, rb[k]);
+            for (int k = 0; k < FB::N; ++k) put_one(TB(), lb, BJ * BR, k * THREADS + tid, rb[k], &largest_b);
         },
         [&]() {
             s8 fb[TJ][3], ones;
@@ -864,7 +876,8 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
             }
         });
     // 2^-100 in bf16 is 0x0D80
-    bool again = (smallest & 0xFFFFu) < 0x0D7Fu || (smallest >> 16) < 0x0D7Fu;
+    const bool tiny = (smallest & 0xFFFFu) < 0x0D7Fu || (smallest >> 16) < 0x0D7Fu;
+    bool again = false;
 #pragma unroll
     for (int a = 0; a < TI; ++a) {
 #pragma unroll
@@ -873,7 +886,35 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
             for (int e = 0; e < 4; ++e) again |= !(fabsf(acc[a][b][e]) <= 3.402823466e38f);
         again |= !(fabsf(rows[a][0]) <= 3.402823466e38f);
     }
-    if (__syncthreads_or(again)) {
+    again = __syncthreads_or(again || tiny) && [&]() {              // (the same in every thread, from here on)
+        if (__syncthreads_or(again)) return true;
+        float(*most)[2] = (float(*)[2])lds;
+        const float a_wave = wave_most(largest_a), b_wave = wave_most(largest_b);
+        if (lane == 0) {
+            most[threadIdx.x >> 6][0] = a_wave;
+            most[threadIdx.x >> 6][1] = b_wave;
+        }
+        __syncthreads();
+        float most_a = 0.f, most_b = 0.f;
+        for (int w = 0; w < THREADS * GROUPS / 64; ++w) {
+            most_a = fmaxf(most_a, most[w][0]);
+            most_b = fmaxf(most_b, most[w][1]);
+        }
+        const float off = (float)q.per * BR * 0x1p-99f, least = off * (most_a + most_b);
+        bool small = false;
+#pragma unroll
+        for (int a = 0; a < TI; ++a) {
+            const bool row = at.i0 + wi + 16 * a + (lane & 15) < q.p.I;
+#pragma unroll
+            for (int b = 0; b < TJ; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    small |= row && at.j0 + wj + TB::index(b, 4 * (lane >> 4) + e) < q.p.J && !(fabsf(acc[a][b][e]) >= least);
+            small |= sums && row && !(fabsf(rows[a][0]) >= off);
+        }
+        return __syncthreads_or(small) != 0;
+    }();
+    if (again) {
         typedef typename FA::TL NA;
         typedef typename FB::TL NB;
         float *na = (float*)la, *nb = na + BI * BR;

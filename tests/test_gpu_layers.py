@@ -505,3 +505,29 @@ def test_views_with_the_sign_beside_them():
     y = linear(x, two)
     (dx,) = torch.autograd.grad(y, x, v)
     assert float(dx) == -6.0
+
+
+@pytest.mark.parametrize("m,k,n", [(200, 512, 190), (130, 1024, 64), (64, 96, 4096)])
+def test_values_that_underflow_among_others(m, k, n):
+    """Values below 2^-100 here and there, in whole rows of x, in whole columns of the weight, rows of zeros: every element to fp32's
+    own error, k roundings of the sum of its products' magnitudes (and k halves of the smallest step)."""
+    from object_detection_amd.layers import linear
+    g = torch.Generator().manual_seed(13)
+    x, w, dy = (torch.randn(*s, generator=g) for s in ((m, k), (n, k), (m, n)))
+    few = torch.rand(m, k, generator=g) < 0.02
+    x[few] *= 2.0 ** -torch.randint(100, 140, (int(few.sum()),), generator=g).float()
+    dy[torch.rand(m, n, generator=g) < 0.02] *= 2.0 ** -118
+    for scenario in range(6):
+        if scenario == 1: x[5] = torch.randn(k, generator=g) * 2.0 ** -120
+        if scenario == 2: x[m - 1] = 2.0 ** -70 * torch.randn(k, generator=g) * 2.0 ** -62
+        if scenario == 3: x[7] = 0.0
+        if scenario == 4: w[3] *= 2.0 ** -119
+        if scenario == 5: dy[:, 2] = dy[:, 2].sign() * 2.0 ** -121
+        gx, gw, gb = leaves(x, w, torch.zeros(n))
+        y = linear(gx, gw, gb)
+        y.backward(dy.cuda())
+        x64, w64, dy64 = x.double(), w.double(), dy.double()
+        for got, a, b, terms in ((y, x64, w64.t(), k), (gx.grad, dy64, w64, n), (gw.grad, dy64.t(), x64, m), (gb.grad, dy64.t(), torch.ones(m, 1).double(), m)):
+            want, size = a @ b, a.abs() @ b.abs()
+            off = (got.detach().cpu().double().reshape(want.shape) - want).abs()
+            assert bool((off <= (terms + 2) * (size * 2.0 ** -24 + 2.0 ** -150)).all()), (scenario, float((off / size.clamp_min(1e-300)).max()))
