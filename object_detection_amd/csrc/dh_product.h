@@ -763,7 +763,8 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS) k_product_any(const Lau
 // found out and done again with those: a part of an infinity or NaN, or of a value that rounds to an infinity in bf16, leaves a
 // sum that is not finite; a part of a value below 2^-100 may underflow, which is looked for when the values are split.  Such a value
 // is off by 2^-124 at most, its product by that times the other operand's largest: sums that reach 2^25 times what R of
-// those add up to need nothing (a few underflowing gradients among others; without this a tile that held one took twice as long).
+// those add up to need nothing.  (Underflowing gradients here and there in 8192 x 1024 -> 4096: 366 us against 358 without any, and 848 when
+// every tile that holds one is done again.)
 // Six products at 1/16 of the cost each: at best 2.7 times the fp32 rate; the split costs 7 vector instructions per value and
 // tile, which other workgroups' products hide.
 struct Split {
@@ -791,8 +792,8 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest, uint32_t* large
 }
 
 // fp32 products, six bf16 ones each (above).  Long reductions are bound by the vector instructions that split beside the matrix
-// instructions that multiply: 8192 x 1024 -> 4096 353 us = 195 TFLOP/s, 8192^3 198, where the card's fp32 matrix instructions end at
-// 157.  The head's levels at batch 64 (733 MB of 916 written) take 404 us: 266 of memory and 283 of products, which overlap between
+// instructions that multiply: 8192 x 1024 -> 4096 357 us = 193 TFLOP/s, 8192^3 195, where the card's fp32 matrix instructions end at
+// 157.  The head's levels at batch 64 (548 MB of 915 written) take 400 us: 266 of memory and 283 of products, which overlap between
 // the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
 __device__ __forceinline__ float wave_most(uint32_t pair)        // above the magnitude of every value whose first parts made `pair`
 {
