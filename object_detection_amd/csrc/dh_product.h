@@ -1111,7 +1111,7 @@ constexpr int SPLIT = -1;              // stages of a shape whose fp32 values ar
 struct Shape { int bi, bj, br, stages, groups = 1; };
 
 // Tiles (i, j), bytes of a reduction step, waves along i and j, stages of the ring, waves per SIMD
-#define DH_SHAPES(X) X(128, 128, 128, 2, 2, 2, 2) X(128, 128, 64, 2, 2, 3, 3) X(64, 64, 128, 2, 2, 2, 4)
+#define DH_SHAPES(X) X(128, 128, 128, 2, 2, 2, 2) X(128, 128, 64, 2, 2, 3, 3) X(64, 64, 128, 2, 2, 2, 4) X(64, 64, 128, 2, 2, 4, 2)
 #define DH_SHAPES_16(X) X(256, 256, 128, 2, 4, 2, 2)
 
 template <typename T, bool ARC, bool BRC>

@@ -14,10 +14,12 @@ namespace {
 //     overlap between workgroups: the head's levels (128 to 512 channels) at batch 64 119 against 159.
 //   64 x 64 where 128 x 128 would leave CUs without a tile, unless the reduction can be cut into 16 or more steps for two
 //     workgroups per CU: the head's weight gradients at batch 64 (14 tiles, 44 steps each) 117 against 155, 1024 x 1024 over 8192 rows
-//     (16 steps) 34 against 45; but 128 x 128 over 64 x 80 x 80 cells (12 steps) 56 against 40.
+//     (16 steps) 34 against 45; but 128 x 128 over 64 x 80 x 80 cells (12 steps) 56 against 40.  Their ring has 4 stages where there are two
+//     of them per CU at most and a step waits for memory (256 x 4096 -> 4096 26 against 35, 1024 x 4096 -> 1024 26 against 35), 2
+//     where more than two share a CU, whose LDS would hold no more of the deep ones (1024 x 1024 -> 2880, 720 tiles: 14 against 19).
 Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
 {
-    int64_t huge = 0, large = 0, held = 0, tile_steps = 0;
+    int64_t huge = 0, large = 0, small = 0, held = 0, tile_steps = 0;
     const int64_t br = dtype == DH_F32 ? 32 : 64;
     int longest = 0, shortest = 1 << 30;
     for (int w = 0; w < n; ++w) {
@@ -25,17 +27,21 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
         huge += (int64_t)((ps[w].I + 255) / 256) * ((ps[w].J + 255) / 256) * b;
         const int64_t tiles = (int64_t)((ps[w].I + 127) / 128) * ((ps[w].J + 127) / 128) * b;
         large += tiles;
+        small += (int64_t)((ps[w].I + 63) / 64) * ((ps[w].J + 63) / 64) * b;
         tile_steps += tiles * ((ps[w].R + br - 1) / br) * (ps[w].reduce_batch ? ps[w].batch : 1);
         held += (int64_t)ps[w].I * ps[w].J * b;
         if (ps[w].R > longest) longest = ps[w].R;
         if (ps[w].R < shortest) shortest = ps[w].R;
     }
-    // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs
+    // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs, or rows
+    // so short that a workgroup is done with all of them soon (us, bf16: 1 x 4096 -> 1024 6.7 against 9.6 on tiles, 32 x 1000 -> 777 4.8
+    // against 10.3, 1 x 512 -> 512 2.9 against 6.2, fp32 3.6 against 13.9; but 32 x 4096 -> 1024 13 against 10, 1 x 16384 -> 16 19 against 10)
     const dh_product& p = ps[0];
-    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 && (int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2)
+    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 &&
+        ((int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2 || (p.R <= 4096 && (int64_t)p.I * p.R <= 65536)))
         return Shape{0, 16, 128, 1};
     const bool split = dtype == DH_F32 && shortest >= 64;
-    if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, split ? SPLIT : 2};
+    if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, split ? SPLIT : small <= 2 * CUS ? 4 : 2};
     if (split) return Shape{128, 128, 128, SPLIT};
     if (!aligned) return Shape{128, 128, 128, 1};
     if (dtype != DH_F32 && huge >= 2 * CUS && shortest >= 512 && held * 8 >= huge * 65536 * 7) return Shape{256, 256, 128, 2};
@@ -65,8 +71,10 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     int64_t total = 0;
     size_t bytes = 0;
     int64_t all_tiles = 0, tile_steps = 0;
+    bool brief = true;                      // no reduction of more than 2 KB of a row
     for (int w = 0; w < n && t.bi; ++w) {
         const dh_product& p = ps[w];
+        brief = brief && p.R * size * (p.reduce_batch ? p.batch : 1) <= 2048;
         const int64_t tiles = (int64_t)((p.I + t.bi - 1) / t.bi) * ((p.J + t.bj - 1) / t.bj) * (p.reduce_batch ? 1 : p.batch);
         all_tiles += tiles;
         tile_steps += tiles * ((p.R + br - 1) / br) * (p.reduce_batch ? p.batch : 1);
@@ -78,12 +86,14 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     if (grouped) shape->groups = 2;
     // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
     // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each (1024^3 bf16, 256
-    // tiles of 64 x 64, uncut: 11 us against 17).  About as many tiles as CUs are cut too where the reduction is long: one workgroup of a
+    // tiles of 64 x 64, uncut: 11 us against 17), and nothing is cut that the deep ring passes in 16 steps (33 x 1024 -> 4096 9.3 against
+    // 10.2, 1024 x 1000 -> 777 10.2 against 15.1; in 32 steps 33 x 2048 -> 512 12.6 against 10.6).  About as many tiles as CUs are cut too where the reduction is long: one workgroup of a
     // CU has nothing beside it while it waits (4096 x 1024 over 8192 rows, 256 tiles of 128 x 128: bf16 78 us against 102, fp32 377
     // against 544).
     const int64_t once = 2 * CUS;
     int64_t each = (tile_steps + once - 1) / once;
-    const bool cutting = t.bi && !grouped && (all_tiles < CUS || (t.bi == 128 && all_tiles <= CUS * 5 / 4 && each >= 4096 / t.br));
+    const bool cutting = t.bi && !grouped && !(brief && t.stages == 4) &&
+                         (all_tiles < CUS || (t.bi == 128 && all_tiles <= CUS * 5 / 4 && each >= 4096 / t.br));
     if (each < 1024 / t.br) each = 1024 / t.br;
     int order[DH_MAX_PRODUCTS];
     for (int w = 0; w < n; ++w) {          // long reductions first: their workgroups are the ones a launch waits for

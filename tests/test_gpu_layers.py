@@ -531,3 +531,18 @@ def test_values_that_underflow_among_others(m, k, n):
             want, size = a @ b, a.abs() @ b.abs()
             off = (got.detach().cpu().double().reshape(want.shape) - want).abs()
             assert bool((off <= (terms + 2) * (size * 2.0 ** -24 + 2.0 ** -150)).all()), (scenario, float((off / size.clamp_min(1e-300)).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("k", [8, 64, 72, 128, 192, 200, 256, 320, 1016, 1024, 1032, 4096])
+def test_reductions_shorter_and_longer_than_the_ring(dtype, k):
+    """One step and less to many of them, whole and partial last ones, on few tiles, in all three products."""
+    check_rows(72, k, 136, dtype, "silu", True, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 4096, 1024), (32, 2048, 80), (32, 2049, 80), (32, 2048, 1), (16, 4096, 16), (17, 4096, 16),
+                                   (1, 1, 1), (32, 1000, 777), (1, 65536, 3), (2, 65536, 3)])
+def test_few_rows_and_few_outputs(dtype, m, k, n):
+    """Either side of where a few rows stop being worked on straight from memory."""
+    check_rows(m, k, n, dtype, "sigmoid", True, False)
