@@ -75,14 +75,27 @@ template <bool OUT> __device__ __forceinline__ int find(const Table<OUT>& t, int
     return lo;
 }
 
+// A workgroup's chunks, `begin` to `end`: consecutive ones, so that the table is searched once and then followed.
+struct Run {
+    int begin, end, k;
+};
+template <bool OUT> __device__ __forceinline__ Run run_of(const Table<OUT>& t)
+{
+    const int64_t all = t.first[t.count];
+    const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
+    return {begin, end, find(t, begin)};
+}
+
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) k_grad_power(const Table<false> t, double* __restrict__ partial)
 {
     constexpr int V = 16 / sizeof(T);
     __shared__ double shared[4];
     double sum = 0.0;
-    for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const int k = find(t, c);
+    Run run = run_of(t);
+    for (int c = run.begin; c < run.end; ++c) {
+        while (c >= t.first[run.k + 1]) ++run.k;
+        const int k = run.k;
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
         const int n = t.length(k, c);
@@ -152,8 +165,11 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table<OUT> t, const dou
     // as two floats: a factor near the end of fp32's range (norms of 1e38 do not leave it) would lose its bits in one
     const double both = factor / by;
     const float f2 = both < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(f2 == 1.f ? both : both * 0x1p64);
-    for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
-        const int k = find(t, c);
+    if (!OUT && f == 1.f && f2 == 1.f) return;
+    Run run = run_of(t);
+    for (int c = run.begin; c < run.end; ++c) {
+        while (c >= t.first[run.k + 1]) ++run.k;
+        const int k = run.k;
         if (f == 1.f && f2 == 1.f && t.in[k] == t.out(k)) continue;   // in place and nothing to do
         const int64_t at = (int64_t)(c - t.first[k]) * CHUNK;
         const T* g = (const T*)t.in[k] + at;
