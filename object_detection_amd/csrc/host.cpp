@@ -563,7 +563,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
                      (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)))
             fail(std::string(where) + ": an output must have its gradient's number of elements and device, and its type or fp32");
         // elements in one piece and in the order they are read in, or through a copy
-        const bool direct = !o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) || (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides()));
+        const bool direct = read[k].is_same(o) || (!o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) || (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides())));
         written.push_back(direct ? o : at::empty_like(read[k], read[k].options().dtype(o.scalar_type())));
         copies |= !direct;
     }
@@ -603,6 +603,18 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
     return out;
 }
 
+// clip() in place on what the parameters' .grad hold; nothing where none has one.
+std::optional<Tensor> clip_parameters(const char* where, const variable_list& parameters, double limit, int norm, const py::object& scale,
+                                      const py::object& reduce)
+{
+    variable_list grads;
+    grads.reserve(parameters.size());
+    for (const Tensor& p : parameters)
+        if (p.grad().defined()) grads.push_back(p.grad());
+    if (grads.empty()) return std::nullopt;
+    return clip(where, grads, std::nullopt, limit, norm, scale, reduce);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m)
@@ -612,4 +624,5 @@ PYBIND11_MODULE(_host, m)
     m.def("head_convs", &head_convs);
     m.def("total_norm", &total_norm);
     m.def("clip", &clip);
+    m.def("clip_parameters", &clip_parameters);
 }

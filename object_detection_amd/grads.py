@@ -74,6 +74,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     code, limit = _norm_code("clip_grad_norm_", norm_type), _limit("clip_grad_norm_", max_norm)
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     parameters = list(parameters)
+    if group is None and not error_if_nonfinite:
+        norm = L.host().clip_parameters("clip_grad_norm_", parameters, limit, code, scale, None)
+        return torch.zeros(()) if norm is None else norm
     grads = [g for g in [p.grad for p in parameters] if g is not None]
     if not grads and group is not None:         # this rank has nothing to add, the others wait for it all the same
         if not parameters:
