@@ -1,9 +1,9 @@
 // Norm of many gradients taken as one vector, and their scaling by min(1, max_norm / (norm + 1e-6)).
 //
-// Two launches for (up to) 280 tensors, whatever their sizes (176 where the results go to other tensors): the first sums |g|^p into one double per workgroup, the second
-// adds those sums in their order -- every workgroup for itself, 8 KB that sit in L2 -- and scales.  Both are bound by the bytes
-// of the gradients: the factor needs the norm of all of them, so they are read twice.  Sums are doubles from the first element
-// on: a square of an fp32 gradient may leave fp32's range, and a sum over 10^8 elements needs more than 24 bits.  No atomics:
+// Two launches for (up to) 280 tensors, whatever their sizes (176 where the results go to other tensors): the first sums |g|^p into
+// one double per workgroup, the second adds those sums in their order -- every workgroup for itself, 8 KB that sit in L2 -- and
+// scales.  Both are bound by the bytes of the gradients: the factor needs the norm of all of them, so they are read twice (unless
+// they are in place and the factor is 1).  Sums are doubles from the first element on: a square of an fp32 gradient may leave fp32's range, and a sum over 10^8 elements needs more than 24 bits.  No atomics:
 // the result does not depend on the order in which workgroups run.
 //
 // 2^29 elements in 64 tensors: the norm 6.1 TB/s (fp32 351 us, bf16 175), the norm and the scaled copy 5.4 and 5.2 TB/s over the

@@ -563,7 +563,9 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
                      (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat)))
             fail(std::string(where) + ": an output must have its gradient's number of elements and device, and its type or fp32");
         // elements in one piece and in the order they are read in, or through a copy
-        const bool direct = read[k].is_same(o) || (!o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) || (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides())));
+        const bool direct = read[k].is_same(o) ||
+                            (!o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) ||
+                                             (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides())));
         written.push_back(direct ? o : at::empty_like(read[k], read[k].options().dtype(o.scalar_type())));
         copies |= !direct;
     }

@@ -2,7 +2,8 @@
 
 What stands between ComputeLoss / the layers' gradients and the optimizer in a step of object_detection/yolov5/train.py:337-346
 (scaler.scale(loss).backward(); scaler.step(optimizer)): the gradients carry a loss scale there, which both calls can take out on
-the way.  Two launches for up to 280 tensors of one type (176 with other tensors for the results), no host synchronisation, sums in double, results repeat bit for bit.
+the way.  Two launches for up to 280 tensors of one type (176 with other tensors for the results), no host synchronisation, sums
+in double, results repeat bit for bit.
 """
 import torch
 
