@@ -950,7 +950,9 @@ template <typename T> __device__ __forceinline__ void finish_one(const dh_produc
 // waves take the reduction in turns of 128 bytes, fragments come from memory straight into registers (no row is used twice, so
 // LDS would only add a trip), and the waves' sums are added in order at the end.  Lane (m, g) reads 32 consecutive bytes of row
 // m, for two products of which each pairs the same reduction values of A and B; which values those are does not matter.
+// Short products of more rows take it too, 64 rows to a workgroup.
 // One token, 4096 -> 16384 bf16: 24 us = 5.5 TB/s of weight; 4096 -> 4096 7.1 us = 4.7 TB/s (and 16 tokens 9.4).
+constexpr int THIN_ROWS = 64;           // of A that a workgroup takes (16 MI, where there are no more)
 template <typename T, int MI>
 __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
 {
@@ -958,13 +960,13 @@ __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
     __shared__ float sums[WAVES][MI * 256];
     const Plan& q = L.plan[0];
     const dh_product& p = q.p;
-    const int tile = (int)blockIdx.x % q.tiles_j, ob = (int)blockIdx.x / q.tiles_j;
+    const int tile = (int)blockIdx.x % q.tiles_j, rest = (int)blockIdx.x / q.tiles_j, ob = rest / q.tiles_i, i0 = rest % q.tiles_i * THIN_ROWS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, m = lane & 15, g = lane >> 4, R = p.R, j0 = tile * 16;
     const T* b = (const T*)p.b + (int64_t)ob * p.b_batch + (int64_t)(j0 + m < p.J ? j0 + m : p.J - 1) * p.ldb;
     const T* a[MI];
 #pragma unroll
     for (int n = 0; n < MI; ++n)
-        a[n] = (const T*)p.a + (int64_t)ob * p.a_batch + (int64_t)(16 * n + m < p.I ? 16 * n + m : p.I - 1) * p.lda;
+        a[n] = (const T*)p.a + (int64_t)ob * p.a_batch + (int64_t)(i0 + 16 * n + m < p.I ? i0 + 16 * n + m : p.I - 1) * p.lda;
     f4 acc[MI];
 #pragma unroll
     for (int n = 0; n < MI; ++n) acc[n] = f4{0.f, 0.f, 0.f, 0.f};
@@ -1028,12 +1030,14 @@ __global__ void __launch_bounds__(512) k_product_thin(const Launch L)
 #pragma unroll
     for (int n = 0; n < MI; ++n) *reinterpret_cast<f4*>(&sums[wave][n * 256 + m * 16 + 4 * g]) = acc[n];
     __syncthreads();
-    const int i = threadIdx.x / 16, j = j0 + threadIdx.x % 16;
-    if (threadIdx.x >= MI * 256 || i >= p.I || j >= p.J) return;
-    float v = 0.f;
+    for (int k = threadIdx.x; k < MI * 256; k += 512) {
+        const int i = i0 + k / 16, j = j0 + k % 16;
+        if (i >= p.I || j >= p.J) return;
+        float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) v += sums[w][threadIdx.x];
-    finish_one<T>(p, L.act, ob, i, j, v);
+        for (int w = 0; w < WAVES; ++w) v += sums[w][k];
+        finish_one<T>(p, L.act, ob, i, j, v);
+    }
 }
 
 // Sums the partial products of the workgroups along the reduction, in a fixed order, and finishes them.  A thread adds four
@@ -1123,7 +1127,8 @@ void launch_tiles(const Launch& L, bool aligned, const Shape& t, hipStream_t st)
         if constexpr (ARC && BRC) {
             const dim3 all((unsigned)L.plan[0].count);
             if (L.plan[0].p.I <= 16) hipLaunchKernelGGL((k_product_thin<T, 1>), all, dim3(512), 0, st, L);
-            else hipLaunchKernelGGL((k_product_thin<T, 2>), all, dim3(512), 0, st, L);
+            else if (L.plan[0].p.I <= 32) hipLaunchKernelGGL((k_product_thin<T, 2>), all, dim3(512), 0, st, L);
+            else hipLaunchKernelGGL((k_product_thin<T, 4>), all, dim3(512), 0, st, L);
         }
         return;
     }

@@ -33,13 +33,17 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
         if (ps[w].R > longest) longest = ps[w].R;
         if (ps[w].R < shortest) shortest = ps[w].R;
     }
-    // thin: one product, both operands along the reduction, at most 32 rows, and enough groups of 16 outputs for half the CUs, or rows
+    // thin: one product, both operands along the reduction.  At most 32 rows, and enough groups of 16 outputs for half the CUs, or rows
     // so short that a workgroup is done with all of them soon (us, bf16: 1 x 4096 -> 1024 6.7 against 9.6 on tiles, 32 x 1000 -> 777 4.8
-    // against 10.3, 1 x 512 -> 512 2.9 against 6.2, fp32 3.6 against 13.9; but 32 x 4096 -> 1024 13 against 10, 1 x 16384 -> 16 19 against 10)
+    // against 10.3, 1 x 512 -> 512 2.9 against 6.2, fp32 3.6 against 13.9; but 32 x 4096 -> 1024 13 against 10, 1 x 16384 -> 16 19 against 10).
+    // More rows, in groups of 64, where the reduction is short and the CUs hold all groups at once (64 x 512 -> 512 bf16 5.2 against 6.6,
+    // fp32 7.6 against 15.0; 256 x 1024 -> 1024 7.8 against 9.4, fp32 12.6 against 18.1; but 64 x 1024 -> 16384, 1024 groups, 23 against 11)
     const dh_product& p = ps[0];
-    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum && p.I <= 32 &&
-        ((int64_t)((p.J + 15) / 16) * p.batch >= CUS / 2 || (p.R <= 4096 && (int64_t)p.I * p.R <= 65536)))
-        return Shape{0, 16, 128, 1};
+    if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum) {
+        const int64_t groups = (int64_t)((p.J + 15) / 16) * p.batch, all = groups * ((p.I + THIN_ROWS - 1) / THIN_ROWS);
+        if (p.I <= 32 ? groups >= CUS / 2 || (p.R <= 4096 && (int64_t)p.I * p.R <= 65536) : all <= CUS && p.R <= 1024)
+            return Shape{0, 16, 128, 1};
+    }
     const bool split = dtype == DH_F32 && shortest >= 64;
     if (large < CUS && tile_steps < 16 * 2 * CUS) return Shape{64, 64, 128, split ? SPLIT : small <= 2 * CUS ? 4 : 2};
     if (split) return Shape{128, 128, 128, SPLIT};
@@ -105,7 +109,7 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
         const dh_product& p = ps[order[w]];
         Plan& q = L->plan[w];
         q.p = p;
-        q.tiles_i = t.bi ? (p.I + t.bi - 1) / t.bi : p.I > 0;
+        q.tiles_i = t.bi ? (p.I + t.bi - 1) / t.bi : (p.I + THIN_ROWS - 1) / THIN_ROWS;
         q.tiles_j = (p.J + t.bj - 1) / t.bj;
         q.batch_steps = (int)((p.R + br - 1) / br);
         const int64_t steps = (int64_t)q.batch_steps * (p.reduce_batch ? p.batch : 1);

@@ -546,3 +546,11 @@ def test_reductions_shorter_and_longer_than_the_ring(dtype, k):
 def test_few_rows_and_few_outputs(dtype, m, k, n):
     """Either side of where a few rows stop being worked on straight from memory."""
     check_rows(m, k, n, dtype, "sigmoid", True, False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(33, 512, 512), (64, 1024, 16), (65, 1023, 17), (127, 40, 100), (128, 1, 1), (129, 7, 260), (256, 512, 1024),
+                                   (257, 1024, 816), (300, 96, 800), (1024, 1024, 256), (1025, 1024, 240), (4097, 33, 48), (64, 1025, 64)])
+def test_short_products_of_some_rows(dtype, m, k, n):
+    """Groups of 64 rows, whole and partial, either side of where tiles take over."""
+    check_rows(m, k, n, dtype, "silu", True, True)
