@@ -37,11 +37,12 @@ Shape shape_of(const dh_product* ps, int n, int dtype, bool aligned)
     // so short that a workgroup is done with all of them soon (us, bf16: 1 x 4096 -> 1024 6.7 against 9.6 on tiles, 32 x 1000 -> 777 4.8
     // against 10.3, 1 x 512 -> 512 2.9 against 6.2, fp32 3.6 against 13.9; but 32 x 4096 -> 1024 13 against 10, 1 x 16384 -> 16 19 against 10).
     // More rows, in groups of 64, where the reduction is short and the CUs hold all groups at once (64 x 512 -> 512 bf16 5.2 against 6.6,
-    // fp32 7.6 against 15.0; 256 x 1024 -> 1024 7.8 against 9.4, fp32 12.6 against 18.1; but 64 x 1024 -> 16384, 1024 groups, 23 against 11)
+    // fp32 7.6 against 15.0; 256 x 1024 -> 1024 7.8 against 9.4, fp32 12.6 against 18.1; but 64 x 1024 -> 16384, 1024 groups, 23 against 11);
+    // fp32, whose tiles split their values first, up to two groups per CU (512 x 512 -> 1024 12.7 against 17.4, 768 rows 17.5 against 16.7).
     const dh_product& p = ps[0];
     if (n == 1 && p.a_by_reduction && p.b_by_reduction && !p.reduce_batch && !p.a_sum) {
         const int64_t groups = (int64_t)((p.J + 15) / 16) * p.batch, all = groups * ((p.I + THIN_ROWS - 1) / THIN_ROWS);
-        if (p.I <= 32 ? groups >= CUS / 2 || (p.R <= 4096 && (int64_t)p.I * p.R <= 65536) : all <= CUS && p.R <= 1024)
+        if (p.I <= 32 ? groups >= CUS / 2 || (p.R <= 4096 && (int64_t)p.I * p.R <= 65536) : all <= (dtype == DH_F32 ? 2 : 1) * CUS && p.R <= 1024)
             return Shape{0, 16, 128, 1};
     }
     const bool split = dtype == DH_F32 && shortest >= 64;
