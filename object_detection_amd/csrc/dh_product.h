@@ -1357,7 +1357,9 @@ int launch_slope(const void* dy, const void* z, void* dz, void* dbias, int64_t o
     if (split > (outer + 3) / 4) split = (outer + 3) / 4;
     if (split > BIAS_SPLIT) split = BIAS_SPLIT;
     if (split < 1) split = 1;
-    if (inner > 1)
+    if (outer == 0 || inner == 0)               // nothing to read: dbias becomes the sum of no parts
+        split = 0;
+    else if (inner > 1)
         hipLaunchKernelGGL((k_slope_planes<T>), dim3((unsigned)(columns * split)), dim3(256), 0, st, (const T*)dy, (const T*)z, (T*)dz,
                            partial, outer, n, inner, act, (int)split);
     else

@@ -211,6 +211,7 @@ extern "C" int dh_product_slope(const void* dy, const void* z, void* dz, void* d
     if (n >= (1ll << 24) || outer >= (1ll << 40) || inner >= (1ll << 40)) return DH_ERR_ARG;
     int64_t per, all;
     if (__builtin_mul_overflow(outer, inner, &per) || __builtin_mul_overflow(per, n, &all) || all >= (1ll << 60)) return DH_ERR_ARG;
+    if (per == 0 && !dbias) return DH_OK;
     if (per > 0 && (!dy || (z && !dz))) return DH_ERR_ARG;
     if (dbias && (!workspace || workspace_bytes < dh_product_slope_workspace(n))) return DH_ERR_WORKSPACE;
     if (dbias && !dh_aligned16(workspace)) return DH_ERR_ALIGN;

@@ -554,3 +554,39 @@ def test_few_rows_and_few_outputs(dtype, m, k, n):
 def test_short_products_of_some_rows(dtype, m, k, n):
     """Groups of 64 rows, whole and partial, either side of where tiles take over."""
     check_rows(m, k, n, dtype, "silu", True, True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("b,ny,nx", [(2, 0, 5), (2, 5, 0), (0, 4, 5), (0, 0, 0), (3, 0, 1)])
+def test_maps_without_cells(b, ny, nx, act, dtype):
+    """No images, or images without cells: zero gradients for what is trained, all of it together and each alone."""
+    from object_detection_amd.layers import head_convs, pointwise_conv
+    for trained in ((0, 1, 2, 3), (0,), (1,), (2,), (1, 2)):
+        t = [made((b, 8, ny, nx), dtype, 1), made((16, 8, 1, 1), dtype, 2), made((16,), dtype, 3), made((b, 16, ny, nx), dtype, 4)]
+        t = [v.cuda().requires_grad_(k in trained) for k, v in enumerate(t)]
+        y = pointwise_conv(t[0], t[1], t[2], act, t[3])
+        assert y.shape == (b, 16, ny, nx)
+        y.sum().backward()
+        for k in trained:
+            assert t[k].grad.shape == t[k].shape and not t[k].grad.any()
+    x, w, bias = made((b, 8, ny, nx), dtype, 1).cuda(), made((16, 8), dtype, 2).cuda(), made((16,), dtype, 3).cuda().requires_grad_(True)
+    head_convs([x, x], [w, w], [bias, bias])[1].sum().backward()
+    assert not bias.grad.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_slope_entry_without_elements_writes_zeros(dtype):
+    """dbias of no elements is zero; the buffers beside it, here with room, are neither read (they hold NaN) nor written."""
+    from object_detection_amd import _lib as L
+    code = DTYPES.index(dtype)
+    n, guard = 40, torch.full((4096,), float("nan"), dtype=dtype, device="cuda")
+    ws = torch.full((L.lib().dh_product_slope_workspace(n),), 255, dtype=torch.uint8, device="cuda")
+    for outer, inner in ((3, 0), (0, 1), (0, 9), (0, 0)):
+        for z in (None, guard.data_ptr()):
+            dbias = torch.full((n + 8,), 5.0, dtype=dtype, device="cuda")
+            dz = torch.full((4096,), 3.0, dtype=dtype, device="cuda")
+            assert L.lib().dh_product_slope(guard.data_ptr(), z, dz.data_ptr(), dbias.data_ptr(), outer, n, inner, 2, code, ws.data_ptr(), ws.numel(),
+                                            L.stream()) == 0
+            torch.cuda.synchronize()
+            assert not dbias[:n].any() and (dbias[n:] == 5).all() and (dz == 3).all()

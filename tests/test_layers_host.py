@@ -98,3 +98,11 @@ def test_slope_entry_refuses_extents_whose_product_leaves_64_bits():
     for z in (None, 4096):
         assert L.lib().dh_product_slope(None, z, None, 4096, far, 1 << 20, far, 2, 0, 8192, 1 << 40, None) == -1
     assert L.lib().dh_product_slope(None, None, None, 4096, far, 1 << 23, 1, 0, 0, 8192, 1 << 40, None) == -1
+
+
+def test_slope_entry_has_nothing_to_launch_without_elements():
+    """No rows, or maps without cells, and no bias gradient wanted: the call ends on the host, whatever the addresses."""
+    from object_detection_amd import _lib as L
+    for outer, inner in ((0, 1), (0, 7), (2, 0), (0, 0)):
+        for at in (None, 4096):
+            assert L.lib().dh_product_slope(at, 4096, at, None, outer, 8, inner, 2, 0, None, 0, None) == 0
