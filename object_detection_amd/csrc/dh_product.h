@@ -24,7 +24,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u2 __attribute__((ext_vector_type(2)));
-typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 
@@ -763,14 +762,16 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS) k_product_any(const Lau
 // found out and done again with those: a part of an infinity or NaN, or of a value that rounds to an infinity in bf16, leaves a
 // sum that is not finite; a part of a value below 2^-100 may underflow, which is looked for when the values are split.  Such a value
 // is off by 2^-124 at most, its product by that times the other operand's largest: sums that reach 2^25 times what R of
-// those add up to need nothing.  (Underflowing gradients here and there in 8192 x 1024 -> 4096: 366 us against 358 without any, and 848 when
-// every tile that holds one is done again.)
+// those add up to need nothing; the largest are found by another look at the operands, which only tiles that hold such a value take.
+// (Underflowing gradients here and there in 8192 x 1024 -> 4096: 477 us against 374 without any, and 848 when every tile that holds one
+// is done again.  Keeping the largest beside the split costs every tile 1.6 % and these 380.  Looking for small values at the first parts, which
+// misses those below 2^-134, would be 0.7 % faster.)
 // Six products at 1/16 of the cost each: at best 2.7 times the fp32 rate; the split costs 7 vector instructions per value and
 // tile, which other workgroups' products hide.
 struct Split {
     u2 hi, mid, lo;         // four values' parts
 };
-__device__ __forceinline__ Split split(u4 v, uint32_t* smallest, uint32_t* largest)
+__device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
 {
     Split s;
 #pragma unroll
@@ -783,10 +784,9 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest, uint32_t* large
         s.hi[h] = hi;
         s.mid[h] = mid;
         s.lo[h] = __builtin_bit_cast(uint32_t, __builtin_convertvector(t, b2));
-        // the smallest magnitude but zero, per half: 0 - 1 is the largest 16-bit value
-        const us2 size = __builtin_bit_cast(us2, hi & 0x7FFF7FFFu), m = size - us2{1, 1};
-        *smallest = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(us2, *smallest), m));
-        *largest = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, *largest), size));
+        // the smallest magnitude but zero, from the value itself (below 2^-134 its first part is zero too): twice its bits, which
+        // leaves the sign behind, less one; 0 - 1 is the largest number there is
+        *smallest = min(*smallest, min((v[2 * h] << 1) - 1, (v[2 * h + 1] << 1) - 1));
     }
     return s;
 }
@@ -795,10 +795,16 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest, uint32_t* large
 // instructions that multiply: 8192 x 1024 -> 4096 357 us = 193 TFLOP/s, 8192^3 195, where the card's fp32 matrix instructions end at
 // 157.  The head's levels at batch 64 (548 MB of 915 written) take 400 us: 266 of memory and 283 of products, which overlap between
 // the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
-__device__ __forceinline__ float wave_most(uint32_t pair)        // above the magnitude of every value whose first parts made `pair`
+// The largest magnitude in a wave's values (a NaN is passed over: its sums are done again anyway).
+template <int N> __device__ __forceinline__ void most_of(const u4* v, float* most)
 {
-    const uint32_t lo = pair & 0xFFFFu, hi = pair >> 16;
-    float v = __uint_as_float(((lo > hi ? lo : hi) + 1) << 16);
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *most = fmaxf(*most, fabsf(__uint_as_float(v[k][e])));
+}
+__device__ __forceinline__ float wave_most(float v)
+{
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
@@ -825,13 +831,13 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
     f4 acc[TI][TJ], rows[TI];
     clear(acc, rows);
     const bool sums = q.p.a_sum && at.j0 + wj == 0;
-    uint32_t smallest = 0xFFFFFFFFu, largest_a = 0, largest_b = 0;
-    auto put_one = [&](auto tile, __bf16* to, int plane, int k, u4 v, uint32_t* largest) {
+    uint32_t smallest = 0xFFFFFFFFu;
+    auto put_one = [&](auto tile, __bf16* to, int plane, int k, u4 v) {
         typedef decltype(tile) TL;
         constexpr int ROW = TL::ROW_CHUNKS * 2;                     // 4-value pieces in a row
         const int row = k / ROW, c = k % ROW;
         __bf16* o = to + (row * TL::ROW_CHUNKS + ((c >> 1) ^ TL::key(row))) * 8 + (c & 1) * 4;
-        const Split s = split(v, &smallest, largest);
+        const Split s = split(v, &smallest);
         *reinterpret_cast<u2*>(o) = s.hi;
         *reinterpret_cast<u2*>(o + plane) = s.mid;
         *reinterpret_cast<u2*>(o + 2 * plane) = s.lo;
@@ -840,9 +846,9 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
         q, at, group, GROUPS,
         [&](const u4* ra, const u4* rb) {
 #pragma unroll
-            for (int k = 0; k < FA::N; ++k) put_one(TA(), la, BI * BR, k * THREADS + tid, ra[k], &largest_a);
+            for (int k = 0; k < FA::N; ++k) put_one(TA(), la, BI * BR, k * THREADS + tid, ra[k]);
 #pragma unroll
-            for (int k = 0; k < FB::N; ++k) put_one(TB(), lb, BJ * BR, k * THREADS + tid, rb[k], &largest_b);
+            for (int k = 0; k < FB::N; ++k) put_one(TB(), lb, BJ * BR, k * THREADS + tid, rb[k]);
         },
         [&]() {
             s8 fb[TJ][3], ones;
@@ -876,8 +882,7 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
                 }
             }
         });
-    // 2^-100 in bf16 is 0x0D80
-    const bool tiny = (smallest & 0xFFFFu) < 0x0D7Fu || (smallest >> 16) < 0x0D7Fu;
+    const bool tiny = smallest < (0x0D800000u << 1) - 1;            // the bits of 2^-100
     bool again = false;
 #pragma unroll
     for (int a = 0; a < TI; ++a) {
@@ -889,6 +894,9 @@ __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(
     }
     again = __syncthreads_or(again || tiny) && [&]() {              // (the same in every thread, from here on)
         if (__syncthreads_or(again)) return true;
+        float largest_a = 0.f, largest_b = 0.f;
+        pass_over<FA, FB, BR, 1>(
+            q, at, group, GROUPS, [&](const u4* ra, const u4* rb) { most_of<FA::N>(ra, &largest_a); most_of<FB::N>(rb, &largest_b); }, []() {});
         float(*most)[2] = (float(*)[2])lds;
         const float a_wave = wave_most(largest_a), b_wave = wave_most(largest_b);
         if (lane == 0) {
