@@ -6,11 +6,13 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/utils.h>
 
 #include "../../include/dethead.h"
 
 #include <algorithm>
 #include <array>
+#include <memory>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -270,10 +272,10 @@ std::tuple<Tensor, Tensor> slope(bool rows, const Tensor& dy, const Tensor& z, i
     return {dz, dbias};
 }
 
-// Under create_graph the gradients pass through this node: a second derivative is refused, not taken for zero.
-struct Last : torch::autograd::Function<Last> {
-    static Tensor forward(AutogradContext*, const Tensor& gradient, const Tensor&, const Tensor&, const Tensor&) { return gradient.alias(); }
-    static variable_list backward(AutogradContext*, variable_list)
+// Under create_graph the gradients leave through this node, whose edges lead to all that they depend on: a second derivative is
+// refused, not taken for zero.
+struct Last : torch::autograd::Node {
+    variable_list apply(variable_list&&) override
     {
         fail("object_detection_amd.layers: a second derivative of a product is not offered");
     }
@@ -304,9 +306,8 @@ struct Products : torch::autograd::Function<Products> {
         const int arguments = (int)(how % 32), act = (int)(how / 64);
         const bool rows = how / 32 % 2, create_graph = at::GradMode::is_enabled();
         const int64_t present = ctx->saved_data["present"].toInt();
-        const auto wanted = [&](size_t k) {
-            return (present >> k & 1) && ctx->needs_input_grad(__builtin_popcountll(present & ((1ll << k) - 1)));
-        };
+        const auto place_of = [&](size_t k) { return (size_t)__builtin_popcountll(present & ((1ll << k) - 1)); };     // among this node's edges
+        const auto wanted = [&](size_t k) { return (present >> k & 1) && ctx->needs_input_grad(place_of(k)); };
         const at::AutoGradMode off(false);
         const variable_list saved = ctx->get_saved_variables();
         variable_list result(2 + arguments);
@@ -341,10 +342,20 @@ struct Products : torch::autograd::Function<Products> {
         run(inputs, 0, saved[0]);
         run(weights, 0, saved[0]);
         if (create_graph) {
-            const at::AutoGradMode on(true);
-            for (size_t k = 0; k < grads.size(); ++k)
-                for (int e = 0; e < 4; ++e)
-                    if (result[2 + 4 * k + e].defined()) result[2 + 4 * k + e] = Last::apply(result[2 + 4 * k + e], grads[k], saved[3 * k], saved[3 * k + 1]);
+            // the inputs' edges are this node's own: what was saved may be a copy that was made without a graph
+            const auto node = torch::autograd::get_current_node();
+            for (size_t k = 0; k < grads.size(); ++k) {
+                if (!grads[k].defined()) continue;
+                torch::autograd::edge_list edges{torch::autograd::impl::gradient_edge(grads[k])};
+                for (size_t e = 4 * k; e < 4 * k + 3; ++e)
+                    if (present >> e & 1) edges.push_back(node->next_edge(place_of(e)));
+                if (std::none_of(edges.begin(), edges.end(), [](const torch::autograd::Edge& e) { return e.is_valid(); })) continue;
+                const std::shared_ptr<Last> last(new Last, torch::autograd::deleteNode);
+                last->set_next_edges(std::move(edges));
+                for (int e = 0; e < 3; ++e)
+                    if (result[2 + 4 * k + e].defined()) torch::autograd::set_history(result[2 + 4 * k + e], last);
+                if (result[2 + 4 * k + 3].defined()) result[2 + 4 * k + 3] = grads[k];      // the residual's: dy, with its own graph
+            }
         }
         return result;
     }

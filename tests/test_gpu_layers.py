@@ -622,3 +622,53 @@ def test_an_operand_of_nothing_but_the_smallest_values(m, k, n, small, large):
     gw2 = w.cuda().requires_grad_(True)
     linear(big, gw2).backward(dy.cuda())
     hold(gw2.grad, D.t(), big.double(), m, "dw")
+
+
+@pytest.mark.parametrize("act", [None, "silu"])
+@pytest.mark.parametrize("trained", [(0,), (1,), (2,), (0, 1, 2, 3)])
+@pytest.mark.parametrize("layout", ["contiguous", "copied"])
+def test_second_derivatives_are_refused(layout, trained, act):
+    """Through the gradient of each input, also where a copy of the input was read and where nothing else is trained: an error, not a
+    term left out."""
+    from object_detection_amd.layers import head_convs, linear, pointwise_conv
+    def inputs(*shapes):
+        t = [made(s, torch.float32, 60 + k).cuda() for k, s in enumerate(shapes)]
+        if layout == "copied":
+            t = [v.transpose(0, 1).contiguous().transpose(0, 1) if v.dim() > 1 else torch.stack([v, v], 1)[:, 0] for v in t]
+        return [v.requires_grad_(k in trained) for k, v in enumerate(t)]
+    calls = ((linear, inputs((6, 8), (10, 8), (10,), (6, 10))), (pointwise_conv, inputs((2, 8, 3, 4), (10, 8), (10,), (2, 10, 3, 4))))
+    for call, (x, w, b, r) in calls:
+        t = [v for k, v in enumerate((x, w, b, r)) if k in trained]
+        y = call(x, w, b, act, r)
+        grads = torch.autograd.grad(y.sum(), t, create_graph=True)
+        for k, g in zip(trained, grads):
+            if k == 3:                                                  # the residual's gradient is dy itself: constant here
+                assert not g.requires_grad
+                continue
+            with pytest.raises(RuntimeError, match="second derivative"):
+                (y.sum() + g.square().sum()).backward(retain_graph=True)
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad(g.sum(), t, retain_graph=True, allow_unused=True)
+    x, w, b, _ = calls[1][1]
+    if trained != (0, 1, 2, 3):
+        ys = head_convs([x, x.detach()], [w, w.detach()], [b, b.detach()])
+        t = (x, w, b)[trained[0]]
+        g, = torch.autograd.grad(ys[0].sum() + ys[1].sum(), t, create_graph=True)
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(g.sum(), t)
+
+
+def test_a_gradient_of_a_residual_can_be_differentiated():
+    """dr = dy, so what dy depends on can be reached through it; and first derivatives under create_graph are the ordinary ones."""
+    from object_detection_amd.layers import linear
+    x, w, b, r, dy = rows_case(7, 16, 12, torch.float32, "silu", True, True)
+    gx, gw, gb, gr, gdy = leaves(x, w, b, r, dy)
+    y = linear(gx, gw, gb, "silu", gr)
+    dr, dx, dw, db = torch.autograd.grad(y, (gr, gx, gw, gb), gdy, create_graph=True)
+    want = rows64(x, w, b, "silu", r, dy)
+    for got, name in ((dx, "dx"), (dw, "dw"), (db, "db")):
+        close(got, want[name], name)
+    back, = torch.autograd.grad((dr * dr).sum(), gdy, retain_graph=True)
+    assert torch.equal(back, 2 * gdy.detach())
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(dx.sum(), gdy)
