@@ -4,6 +4,7 @@
 // 85 us); everything that computes is in libdethead.
 #include <torch/extension.h>
 #include <ATen/autocast_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -71,6 +72,13 @@ struct Item {
 // The kernels read memory: a view whose sign is kept beside it (the imaginary part of a conjugate) is written out first.
 Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
+// Kernels carry no tangents: a dual tensor is refused, its derivative not taken for zero.
+void refuse_dual(const char* where, const Tensor& t)
+{
+    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+        fail(std::string(where) + ": forward-mode derivatives are not offered");
+}
+
 // One supported type on one ROCm device; under autocast its type.
 void check_tensors(const char* where, Item& it)
 {
@@ -78,6 +86,8 @@ void check_tensors(const char* where, Item& it)
         fail(std::string(where) + ": x is on " + it.x.device().str() + ": object_detection_amd only runs on ROCm devices (no CPU fallback)");
     for (Tensor* t : it.all())
         if (t->defined() && t->is_neg()) *t = t->resolve_neg();
+    for (Tensor* t : it.all())
+        if (t->defined()) refuse_dual(where, *t);
     for (Tensor* t : it.all())
         if (t->defined() && t->device() != it.x.device())
             fail(std::string(where) + ": tensors on " + t->device().str() + " and " + it.x.device().str());
@@ -455,6 +465,7 @@ std::vector<List> listed(const char* where, const variable_list& grads, variable
         if (!g.is_cuda())
             fail(std::string(where) + ": a gradient is on " + g.device().str() + ": object_detection_amd only runs on ROCm devices (no CPU fallback)");
         if (g.layout() != at::kStrided) fail(std::string(where) + ": gradients must be dense tensors");
+        refuse_dual(where, g);
         if (g.device() != grads[0].device()) fail(std::string(where) + ": gradients on " + grads[0].device().str() + " and " + g.device().str());
         const at::ScalarType type = g.scalar_type();
         if (code_of(type) < 0) fail(std::string(where) + ": gradients must be fp32, fp16 or bf16, got " + c10::toString(type));

@@ -672,3 +672,44 @@ def test_a_gradient_of_a_residual_can_be_differentiated():
     assert torch.equal(back, 2 * gdy.detach())
     with pytest.raises(RuntimeError, match="second derivative"):
         torch.autograd.grad(dx.sum(), gdy)
+
+
+@pytest.mark.parametrize("trained", [False, True])
+def test_forward_mode_is_refused(trained):
+    """A dual input, weight, bias or residual: an error, not a result without its tangent.  Where forward mode is off, or the level has
+    ended, the calls run."""
+    import torch.autograd.forward_ad as ad
+    from object_detection_amd.grads import clip_grads, total_grad_norm
+    from object_detection_amd.layers import head_convs, linear, pointwise_conv
+    t = [made(s, torch.float32, 80 + k).cuda().requires_grad_(trained) for k, s in enumerate(((1, 8, 4, 5), (6, 8, 1, 1), (6,), (1, 6, 4, 5)))]
+    rows = [made(s, torch.float32, 90 + k).cuda().requires_grad_(trained) for k, s in enumerate(((20, 8), (6, 8), (6,), (20, 6)))]
+    with ad.dual_level():
+        for k in range(4):
+            dual = [ad.make_dual(v, torch.ones_like(v)) if e == k else v for e, v in enumerate(t)]
+            dual_rows = [ad.make_dual(v, torch.ones_like(v)) if e == k else v for e, v in enumerate(rows)]
+            calls = [lambda: pointwise_conv(*dual[:3], "silu", dual[3]), lambda: linear(*dual_rows[:3], "silu", dual_rows[3])]
+            if k < 3:
+                calls.append(lambda: head_convs([t[0], dual[0]], [t[1], dual[1]], [t[2], dual[2]]))
+            for call in calls:
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+                with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                    call()
+                with ad._set_fwd_grad_enabled(False):
+                    call()
+        g = ad.make_dual(torch.ones(5, device="cuda"), torch.ones(5, device="cuda"))
+        for call in (lambda: total_grad_norm([g]), lambda: clip_grads([g], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+    pointwise_conv(*t[:3], "silu", t[3])
+
+
+def test_forward_mode_of_a_fused_head_is_refused():
+    import torch.autograd.forward_ad as ad
+    from object_detection_amd.yolo import Detect
+    det = Detect(3, [[1, 2, 3, 4]], (8,)).cuda().train()
+    x = torch.randn(1, 8, 5, 6, device="cuda")
+    det.fused_convs = True
+    with ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        det([ad.make_dual(x, torch.ones_like(x))])
+    assert det([x])[0].shape == (1, 2, 5, 6, 8)
