@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from tests._products import close, rows64, to_maps, to_rows
+from tests._products import LOWEST, close, rows64, to_maps, to_rows
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
@@ -713,3 +713,31 @@ def test_forward_mode_of_a_fused_head_is_refused():
     with ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         det([ad.make_dual(x, torch.ones_like(x))])
     assert det([x])[0].shape == (1, 2, 5, 6, 8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ["silu", "gelu", "sigmoid"])
+def test_16_bit_activations_relative_to_their_own_size(act, dtype):
+    """Far out an activation and its slope are small numbers that 16 bits still hold: each to 2^-13 of its terms' magnitudes (the
+    approximations' 2^-14, and arguments up to 126 whose roundings an exponential multiplies, 126 * 2^-24), fp32's own 2^-22 where
+    terms near 1 cancel, one rounding to the type, and what underflows in fp32 (|z| 2^-125)."""
+    from object_detection_amd.layers import linear
+    g = torch.Generator().manual_seed(3)
+    z = torch.cat([torch.linspace(-16, 16, 1501), torch.linspace(-100, 100, 401), torch.rand(2000, generator=g) * 12 - 12]).to(dtype)
+    n = z.numel()
+    for rows, wide in ((n, 1), (1, n)):                     # z = x w with either of them 1: exact
+        x, w = (z[:, None], torch.ones(1, 1, dtype=dtype)) if wide == 1 else (torch.ones(1, 1, dtype=dtype), z[:, None])
+        gx = x.cuda().requires_grad_(wide == 1)
+        y = linear(gx, w.cuda(), activation=act)
+        Z = z.double().reshape(rows, wide)
+        s, tail = torch.special.expit(Z), torch.special.expit(-Z)
+        normal, bell = torch.erfc(-Z * 0.5 ** 0.5) / 2, torch.exp(-Z * Z / 2) * 0.3989422804014327        # (ndtr ends at 1e-16)
+        value = {"silu": Z * s, "gelu": Z * normal, "sigmoid": s}[act]
+        low = LOWEST[dtype]
+        close(y, (value, value.abs() * (2.0 ** -13 + torch.finfo(dtype).eps / 2 * 1.001) + low + Z.abs() * 2.0 ** -125 + 2.0 ** -126), f"{act} value")
+        if wide == 1:
+            y.sum().backward()
+            slope = {"silu": s * (1 + Z * tail), "gelu": normal + Z * bell, "sigmoid": s * tail}[act]
+            terms = {"silu": s * (1 + Z.abs() * (tail + 2.0 ** -9)), "gelu": normal + Z.abs() * bell, "sigmoid": s * tail + s * 2.0 ** -9}[act]
+            close(gx.grad, (slope, terms * 2.0 ** -13 + slope.abs() * torch.finfo(dtype).eps / 2 * 1.001 + low + (1 + Z.abs()) * 2.0 ** -125),
+                  f"{act} slope")
