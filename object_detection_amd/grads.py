@@ -34,18 +34,21 @@ def _over(group, norm_type):
     return lambda power: all_reduce_norm_power(power, float(norm_type), None if group is True else group)
 
 
+def _nothing(parameters=()):
+    """The empty gradient with which a rank that has none takes part in the exchange the others wait in."""
+    return torch.empty(0, device=next((p.device for p in parameters if p.is_cuda), torch.device("cuda")))
+
+
 def total_grad_norm(grads, norm_type=2.0, scale=None, group=None):
     """The norm of all `grads` as one vector: a 0-dim fp32 tensor on their device (0 on the CPU for an empty list).
 
     norm_type 1, 2 or inf; scale: a factor the gradients carry (GradScaler's, a number or a one-element tensor) and the norm is
     to be free of.  group: a process group (True: the default one) over which gradients are sharded -- every rank passes its own
-    shards and gets the norm of all of them; leave it out for replicated gradients."""
+    shards (a rank may have none) and gets the norm of all of them; leave it out for replicated gradients."""
     code, grads = _norm_code("total_grad_norm", norm_type), list(grads)
     if not grads and group is None:
         return torch.zeros(())
-    if not grads:
-        raise RuntimeError("total_grad_norm: a rank of a group needs at least one gradient (it may be empty)")
-    return L.host().total_norm(grads, code, scale, _over(group, norm_type))
+    return L.host().total_norm(grads or [_nothing()], code, scale, _over(group, norm_type))
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, scale=None, out=None, group=None):
@@ -58,7 +61,9 @@ def clip_grads(grads, max_norm, norm_type=2.0, scale=None, out=None, group=None)
     worthless, as after torch's clipping."""
     code, limit, grads = _norm_code("clip_grads", norm_type), _limit("clip_grads", max_norm), list(grads)
     if not grads:
-        raise RuntimeError("clip_grads: no gradients")
+        if group is None or out:
+            raise RuntimeError("clip_grads: no gradients")
+        return total_grad_norm(grads, norm_type, scale, group), []
     if out is None:
         out = [torch.empty_like(g) for g in grads]
     else:
@@ -82,7 +87,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if not grads and group is not None:         # this rank has nothing to add, the others wait for it all the same
         if not parameters:
             raise RuntimeError("clip_grad_norm_: a rank of a group needs at least one parameter")
-        grads = [parameters[0].detach().new_empty(0)]
+        grads = [_nothing(parameters)]
     if not grads:
         return torch.zeros(())
     if error_if_nonfinite:

@@ -383,3 +383,25 @@ def test_training_step_of_the_head():
             for a, b in zip(maps0, maps1):
                 torch.testing.assert_close(a, b, rtol=2e-3 if half else 1e-5, atol=4e-3 if half else 1e-5)
             assert z0.shape == z1.shape and len(d0) == len(d1)
+
+
+def test_a_rank_without_gradients_of_any_kind_takes_part(monkeypatch):
+    """Parameters that the kernels would refuse (double, on the host), and no gradients at all: the exchange the others wait in happens."""
+    from object_detection_amd import grads as G
+    met = []
+
+    def exchange(power, norm_type, group):
+        met.append((float(power), power.is_cuda, norm_type))
+        return power + 9.0
+    monkeypatch.setattr(G, "all_reduce_norm_power", exchange)
+    host, double = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(2, device="cuda", dtype=torch.float64))
+    for parameters in ([host], [double], [host, double]):
+        assert float(G.clip_grad_norm_(parameters, 1.0, group=True)) == 3.0
+        assert float(G.clip_grad_norm_(parameters, 1.0, group=True, error_if_nonfinite=True)) == 3.0
+    assert len(met) == 9
+    assert float(G.total_grad_norm([], group=True)) == 3.0
+    norm, out = G.clip_grads([], 1.0, group=True)
+    assert float(norm) == 3.0 and out == []
+    assert met == [(0.0, True, 2.0)] * 11
+    with pytest.raises(RuntimeError):
+        G.clip_grads([], 1.0)
