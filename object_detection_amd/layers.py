@@ -12,6 +12,7 @@ import ctypes
 
 from . import _lib as L
 
+MAX_LEVELS = 5          # of head_convs(): DH_MAX_PRODUCTS of include/dethead.h
 ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "sigmoid": 4}
 
 

@@ -6,7 +6,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .layers import head_convs
+from .layers import MAX_LEVELS, head_convs
 
 
 _ANCHOR_CACHE = {}
@@ -344,10 +344,37 @@ def clip_augmented(y, nl):
     return y
 
 
+# hooks that torch calls for every module (register_module_forward_hook and the like)
+_GLOBAL_HOOKS = [hooks for hooks in (getattr(nn.modules.module, f"_global_{kind}_hooks", None)
+                                     for kind in ("forward", "forward_pre", "backward", "backward_pre")) if hooks is not None]
+_TYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
 def _plain_conv(m):
     """A 1x1 convolution whose call is its product and nothing else."""
-    return (type(m) is nn.Conv2d and m.kernel_size == (1, 1) and m.stride == (1, 1) and m.padding == (0, 0) and m.groups == 1
-            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks))
+    if (type(m) is not nn.Conv2d or m.kernel_size != (1, 1) or m.stride != (1, 1) or m.padding != (0, 0) or m.groups != 1
+            or m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks):
+        return False
+    for hooks in _GLOBAL_HOOKS:
+        if hooks:
+            return False
+    own = m.__dict__
+    return not ("forward" in own or "_conv_forward" in own or "_call_impl" in own or own.get("_compiled_call_impl"))
+
+
+def _one_launch(xs, convs):
+    """Whether head_convs() computes what the layers would: its number of levels, maps on one device and of one type that it has
+    (autocast makes it one, of all but doubles)."""
+    if not 1 <= len(xs) <= MAX_LEVELS:
+        return False
+    device, one, autocast = xs[0].device, xs[0].dtype, torch.is_autocast_enabled("cuda")
+    for x, m in zip(xs, convs):
+        if not x.is_cuda or x.device != device or x.dim() != 4 or not _plain_conv(m):
+            return False
+        for t in (x, m.weight, m.bias):
+            if t is not None and (t.dtype not in _TYPES or (t.dtype is not one and not autocast)):
+                return False
+    return True
 
 
 class Detect(nn.Module):
@@ -406,9 +433,9 @@ class Detect(nn.Module):
         return grid, anchor_grid
 
     def _convolutions(self, x):
-        """yolo.py:52 for every level.  On the CPU (the pass that derives the strides), for replaced layers and for layers with hooks
-        (pruning and the like rebuild the weight in one), the layers themselves."""
-        if self.fused_convs and all(v.is_cuda for v in x[:self.nl]) and all(_plain_conv(m) for m in self.m):
+        """yolo.py:52 for every level.  On the CPU (the pass that derives the strides), for replaced layers, for layers with hooks
+        (pruning and the like rebuild the weight in one) and for what head_convs() does not take, the layers themselves."""
+        if self.fused_convs and _one_launch(x[:self.nl], self.m):
             return head_convs(x[:self.nl], [m.weight for m in self.m], [m.bias for m in self.m])
         return [self.m[i](x[i]) for i in range(self.nl)]
 

@@ -741,3 +741,59 @@ def test_16_bit_activations_relative_to_their_own_size(act, dtype):
             terms = {"silu": s * (1 + Z.abs() * (tail + 2.0 ** -9)), "gelu": normal + Z.abs() * bell, "sigmoid": s * tail + s * 2.0 ** -9}[act]
             close(gx.grad, (slope, terms * 2.0 ** -13 + slope.abs() * torch.finfo(dtype).eps / 2 * 1.001 + low + (1 + Z.abs()) * 2.0 ** -125),
                   f"{act} slope")
+
+
+def test_a_fused_head_takes_what_its_layers_take():
+    """Six levels, doubles, levels of different types, a patched layer and a module-wide hook: the layers' own results; the ordinary head
+    is one launch."""
+    from object_detection_amd import yolo
+    from object_detection_amd.yolo import Detect
+
+    def head(nl, dtype=torch.float32):
+        det = Detect(3, [[1, 2, 3, 4]] * nl, (8,) * nl).to(device="cuda", dtype=dtype).train()
+        det.fused_convs = True
+        det.lazy_maps = True
+        return det, [made((2, 8, 5 + l, 6), dtype, l).cuda() for l in range(nl)]
+    launches = []
+    real = yolo.head_convs
+    yolo.head_convs = lambda *a: launches.append(1) or real(*a)
+    try:
+        def run(det, xs, fused):
+            del launches[:]
+            got = det._convolutions(list(xs))
+            assert len(launches) == fused
+            for g, m, x in zip(got, det.m, xs):
+                want = m(x)
+                assert g.dtype == want.dtype and g.shape == want.shape
+                if not fused:
+                    assert torch.equal(g, want)
+        for nl, fused in ((1, 1), (3, 1), (5, 1), (6, 0)):
+            run(*head(nl), fused)
+        run(*head(3, torch.float64), 0)
+        det, xs = head(3)
+        det.m[1].double()
+        run(det, [xs[0], xs[1].double(), xs[2]], 0)
+        det, xs = head(2)
+        det.m[1].half()
+        run(det, [xs[0], xs[1].half()], 0)
+        det, xs = head(2)
+        plain = det.m[0].forward
+        det.m[0].forward = lambda x: plain(x) + 1
+        run(det, xs, 0)
+        del det.m[0].forward
+        run(det, xs, 1)
+        seen = []
+        handle = torch.nn.modules.module.register_module_forward_hook(lambda m, *a: seen.append(m))
+        try:
+            run(det, xs, 0)
+        finally:
+            handle.remove()
+        assert det.m[0] in seen and det.m[1] in seen
+        with torch.autocast("cuda", dtype=torch.float16):
+            del launches[:]
+            got = det._convolutions([xs[0], xs[1].half()])
+            assert launches == [1] and all(g.dtype == torch.float16 for g in got)
+        with torch.autocast("cuda", dtype=torch.float16), pytest.raises(RuntimeError):      # as its layers do
+            det._convolutions([xs[0].double(), xs[1]])
+    finally:
+        yolo.head_convs = real

@@ -106,3 +106,35 @@ def test_slope_entry_has_nothing_to_launch_without_elements():
     for outer, inner in ((0, 1), (0, 7), (2, 0), (0, 0)):
         for at in (None, 4096):
             assert L.lib().dh_product_slope(at, 4096, at, None, outer, 8, inner, 2, 0, None, 0, None) == 0
+
+
+def test_a_fused_head_keeps_what_torch_would_call():
+    """Hooks of all modules, a forward, a convolution or a call that an instance brings along: the layer itself runs."""
+    from object_detection_amd.yolo import _plain_conv
+    nn, module = torch.nn, torch.nn.modules.module
+    m = nn.Conv2d(4, 6, 1)
+    for register in (module.register_module_forward_hook, module.register_module_forward_pre_hook, module.register_module_full_backward_hook,
+                     module.register_module_full_backward_pre_hook):
+        handle = register(lambda *a: None)
+        try:
+            assert not _plain_conv(m)
+        finally:
+            handle.remove()
+        assert _plain_conv(m)
+    for name in ("forward", "_conv_forward"):
+        m = nn.Conv2d(4, 6, 1)
+        setattr(m, name, lambda *a: None)
+        assert not _plain_conv(m)
+        delattr(m, name)
+        assert _plain_conv(m)
+    m = nn.Conv2d(4, 6, 1)
+    m.compile()
+    assert not _plain_conv(m)
+    for make in (nn.utils.parametrizations.weight_norm, nn.utils.parametrizations.spectral_norm):
+        assert not _plain_conv(make(nn.Conv2d(4, 6, 1)))
+
+
+def test_the_number_of_levels_is_the_header_s():
+    from object_detection_amd.layers import MAX_LEVELS
+    with open(os.path.join(ROOT, "include", "dethead.h")) as f:
+        assert f"#define DH_MAX_PRODUCTS {MAX_LEVELS}\n" in f.read()
