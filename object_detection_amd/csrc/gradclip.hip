@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) k_grad_join(const double* __restrict__ pa
     const double v = total<KIND>(partial, parts, shared);
     if (threadIdx.x == 0) {
         if (sum) *sum = v;
-        if (norm) *norm = (float)((KIND == DH_NORM_2 ? sqrt(v) : v) / (scale ? (double)*scale : 1.0));
+        if (norm) *norm = (float)((KIND == DH_NORM_2 ? sqrt(v) : v) / (scale ? fabs((double)*scale) : 1.0));
     }
 }
 
@@ -159,13 +159,13 @@ __global__ void __launch_bounds__(256) k_grad_clip(const Table<OUT> t, const dou
     __shared__ double shared[4];
     const double sum = total<KIND>(partial, parts, shared);
     const double by = scale ? (double)*scale : 1.0;
-    const double n_all = (KIND == DH_NORM_2 ? sqrt(sum) : sum) / by;
+    const double n_all = (KIND == DH_NORM_2 ? sqrt(sum) : sum) / fabs(by);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)n_all;
     double factor = max_norm / (n_all + 1e-6);
     factor = factor > 1.0 ? 1.0 : factor;               // (a NaN norm leaves a NaN factor)
     // as two floats: a factor near the end of fp32's range (norms of 1e38 do not leave it) would lose its bits in one
     const double both = factor / by;
-    const float f2 = both < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(f2 == 1.f ? both : both * 0x1p64);
+    const float f2 = fabs(both) < 0x1p-100 ? 0x1p-64f : 1.f, f = (float)(f2 == 1.f ? both : both * 0x1p64);
     if (!OUT && f == 1.f && f2 == 1.f) return;
     Run run = run_of(t);
     for (int c = run.begin; c < run.end; ++c) {

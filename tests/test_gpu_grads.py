@@ -405,3 +405,17 @@ def test_a_rank_without_gradients_of_any_kind_takes_part(monkeypatch):
     assert met == [(0.0, True, 2.0)] * 11
     with pytest.raises(RuntimeError):
         G.clip_grads([], 1.0)
+
+
+@pytest.mark.parametrize("p", [1.0, 2.0, math.inf])
+def test_a_negative_scale(p):
+    """|g / scale| does not depend on the scale's sign, g / scale does."""
+    from object_detection_amd.grads import clip_grads, total_grad_norm
+    grads = made(SHAPES, torch.float32, 21)
+    for scale in (-4.0, torch.tensor([-4.0], device="cuda")):
+        norm = norm64(grads, p, 4.0)
+        near(total_grad_norm(grads, p, scale=scale), norm)
+        for limit in (norm / 2, norm * 2, 1e-38 * norm):
+            n, out = clip_grads(grads, limit, p, scale=scale, out=[torch.empty_like(g) for g in grads])
+            near(n, norm)
+            clipped_close(out, [-g for g in grads], norm, limit, 4.0)
