@@ -3,6 +3,7 @@
 // interpreter needs for the same work is longer than the kernels (a linear call 11 us, a backward 70 us, a list of 111 gradients
 // 85 us); everything that computes is in libdethead.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
@@ -565,6 +566,37 @@ void apart(const char* where, const variable_list& read, const variable_list& wr
     }
 }
 
+// The same for outputs that are written through a copy, `strided` among `into`: no element of their own twice (an expanded tensor), none
+// begins where another begins, and neither their first nor their last element lies in an output that is written directly.
+void strided_apart(const char* where, const variable_list& into, const std::vector<size_t>& strided)
+{
+    std::vector<std::pair<const char*, const char*>> whole;
+    std::vector<bool> copied(into.size());
+    std::vector<const char*> ends, begins;
+    for (const size_t k : strided) {
+        const Tensor& o = into[k];
+        copied[k] = true;
+        if (at::has_internal_overlap(o) == at::MemOverlap::Yes)
+            fail(std::string(where) + ": a gradient or output whose elements share memory (an expanded tensor) cannot be written");
+        if (!o.numel()) continue;
+        int64_t last = 0;
+        for (int64_t d = 0; d < o.dim(); ++d) last += (o.size(d) - 1) * o.stride(d);
+        begins.push_back((const char*)o.data_ptr());
+        ends.push_back(begins.back());
+        ends.push_back(begins.back() + last * (int64_t)o.element_size());
+    }
+    for (size_t k = 0; k < into.size(); ++k)
+        if (!copied[k] && into[k].numel()) whole.push_back({(const char*)into[k].data_ptr(), (const char*)into[k].data_ptr() + into[k].nbytes()});
+    std::sort(begins.begin(), begins.end());
+    std::sort(whole.begin(), whole.end());
+    bool bad = std::adjacent_find(begins.begin(), begins.end()) != begins.end();
+    for (const char* e : ends) {
+        const auto after = std::upper_bound(whole.begin(), whole.end(), e, [](const char* v, const auto& w) { return v < w.first; });
+        bad |= after != whole.begin() && e < (after - 1)->second;
+    }
+    if (bad) fail(std::string(where) + ": a gradient is in the list twice, or two outputs overlap");
+}
+
 // Norm, and outs[k] = grads[k] / scale * factor; without outs in place.
 Tensor clip(const char* where, const variable_list& grads, const std::optional<variable_list>& outs, double limit, int norm,
             const py::object& scale, const py::object& reduce)
@@ -578,7 +610,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
     if (into.size() != grads.size())
         fail(std::string(where) + ": " + std::to_string(grads.size()) + " gradients and " + std::to_string(into.size()) + " outputs");
     const c10::DeviceGuard guard(grads[0].device());
-    bool copies = false;
+    std::vector<size_t> copies;             // outputs that are written through a copy
     for (size_t k = 0; k < into.size(); ++k) {
         const Tensor &o = into[k], &g = grads[k];
         if (outs && (o.device() != g.device() || o.numel() != g.numel() || o.layout() != at::kStrided ||
@@ -589,7 +621,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
                             (!o.is_neg() && ((read[k].is_contiguous() && o.is_contiguous()) ||
                                              (dense(o) && o.sizes() == read[k].sizes() && o.strides() == read[k].strides())));
         written.push_back(direct ? o : at::empty_like(read[k], read[k].options().dtype(o.scalar_type())));
-        copies |= !direct;
+        if (!direct) copies.push_back(k);
     }
     // the lists again, by the outputs' type: both kinds may occur for one kind of gradient
     struct Out {
@@ -599,6 +631,7 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
     };
     std::vector<Out> launches;
     apart(where, read, written, !outs);
+    if (!copies.empty()) strided_apart(where, into, copies);
     for (const List& l : lists)
         for (const at::ScalarType type : {l.type, at::kFloat}) {
             if (type == l.type && !launches.empty() && launches.back().list.type == l.type && launches.back().type == type) continue;
@@ -620,8 +653,8 @@ Tensor clip(const char* where, const variable_list& grads, const std::optional<v
                              (const double*)at_or_null(partial), partial.numel(), (const float*)at_or_null(factor), limit, out.data_ptr<float>(),
                              stream_of(grads[0])),
                 "dh_grad_clip");
-    for (size_t k = 0; copies && k < into.size(); ++k)
-        if (!written[k].is_same(into[k])) into[k].copy_(written[k].sizes() == into[k].sizes() ? written[k] : written[k].reshape(into[k].sizes()));
+    for (const size_t k : copies)
+        into[k].copy_(written[k].sizes() == into[k].sizes() ? written[k] : written[k].reshape(into[k].sizes()));
     for (const Tensor& o : into)            // written through raw pointers: keep the version counters honest
         if (!o.is_inference()) o.unsafeGetTensorImpl()->bump_version();
     return out;

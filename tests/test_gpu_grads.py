@@ -419,3 +419,34 @@ def test_a_negative_scale(p):
             n, out = clip_grads(grads, limit, p, scale=scale, out=[torch.empty_like(g) for g in grads])
             near(n, norm)
             clipped_close(out, [-g for g in grads], norm, limit, 4.0)
+
+
+def test_strided_gradients_that_share_memory_are_refused():
+    """Twice the same columns, an expanded gradient, columns of a tensor that is in the list itself: refused before anything is written.
+    Neighbouring columns are apart."""
+    from object_detection_amd.grads import clip_grads, clip_grad_norm_
+    wide = torch.arange(60, device="cuda", dtype=torch.float32).view(6, 10)
+    kept = wide.clone()
+    row = torch.ones(1, 8, device="cuda")
+
+    def parameters(*grads):
+        ps = [torch.nn.Parameter(torch.zeros(g.shape, device="cuda")) for g in grads]
+        for q, g in zip(ps, grads):
+            q.grad = g
+        return ps
+    for grads, match in (((wide[:, 2:5], wide[:, 2:5]), "twice"), ((wide[:, 2:5], wide[:, 2:4]), "twice"), ((row.expand(4, 8),), "share memory"),
+                         ((wide, wide[:, 3:5]), "overlap"), ((wide[:, 0:3], wide[0:2]), "overlap")):
+        with pytest.raises(RuntimeError, match=match):
+            clip_grad_norm_(parameters(*grads), 1.0)
+        with pytest.raises(RuntimeError, match=match):
+            clip_grads([torch.ones(g.shape, device="cuda") for g in grads], 1.0, out=list(grads))
+    assert torch.equal(wide, kept) and (row == 1).all()
+    grads = [wide[:, 0:2], wide[:, 2:5], wide[:, 5:9:2]]
+    before = [g.clone() for g in grads]
+    norm = norm64(before, 2.0)
+    near(clip_grad_norm_(parameters(*grads), 3.0), norm)
+    clipped_close(grads, before, norm, 3.0)
+    assert torch.equal(wide[:, 9], kept[:, 9]) and torch.equal(wide[:, 6:9:2], kept[:, 6:9:2])
+    # read as often as one likes: an expanded gradient counts each of its elements, into other tensors
+    n, out = clip_grads([row.expand(4, 8), wide[:, 2:5], wide[:, 2:5]], 1e9)
+    near(n, norm64([row.expand(4, 8), wide[:, 2:5], wide[:, 2:5]], 2.0))
