@@ -92,9 +92,11 @@ int cut(const dh_product* ps, int n, int dtype, Launch* L, float* ws, size_t* ws
     // Fewer tiles than CUs: reductions are cut so that every workgroup of the launch has about the same number of steps, two
     // workgroups per CU.  Joining costs a launch and two passes over the partial sums, so at least 1 KB of a row each (1024^3 bf16, 256
     // tiles of 64 x 64, uncut: 11 us against 17), and nothing is cut that the deep ring passes in 16 steps (33 x 1024 -> 4096 9.3 against
-    // 10.2, 1024 x 1000 -> 777 10.2 against 15.1; in 32 steps 33 x 2048 -> 512 12.6 against 10.6).  About as many tiles as CUs are cut too where the reduction is long: one workgroup of a
-    // CU has nothing beside it while it waits (4096 x 1024 over 8192 rows, 256 tiles of 128 x 128: bf16 78 us against 102, fp32 377
-    // against 544).
+    // 10.2, 1024 x 1000 -> 777 10.2 against 15.1; in 32 steps 33 x 2048 -> 512 12.6 against 10.6).  The same holds for operands of any
+    // alignment, which have no ring but as short a reduction (256 x 777 -> 1501 11.6 against 12.6, 300 x 1023 -> 2001 13.8 against 16.2,
+    // 601 channels at 1401 x 320 9.5 against 11.8; 1024 -> 255 channels of 13 x 13 cells 12.2 against 11.8).
+    // About as many tiles as CUs are cut too where the reduction is long: one workgroup of a CU has nothing beside it while it waits
+    // (4096 x 1024 over 8192 rows, 256 tiles of 128 x 128: bf16 78 us against 102, fp32 377 against 544).
     const int64_t once = 2 * CUS;
     int64_t each = (tile_steps + once - 1) / once;
     const bool cutting = t.bi && !grouped && !(brief && t.stages == 4) &&
