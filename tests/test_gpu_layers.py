@@ -797,3 +797,61 @@ def test_a_fused_head_takes_what_its_layers_take():
             det._convolutions([xs[0].double(), xs[1]])
     finally:
         yolo.head_convs = real
+
+
+class _Given(torch.nn.Module):
+    """A level's convolution whose output is already there."""
+
+    def __init__(self, conv, out):
+        super().__init__()
+        self.weight, self.bias, self.out = conv.weight, conv.bias, out
+
+    def forward(self, x):
+        return self.out
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("lazy", [False, True])
+def test_a_fused_head_in_eval(lazy, half):
+    """The fused convolutions against 64 bits, what follows them bit for bit what an ordinary head makes of the same maps, in forward() and
+    in detections(), and the decoded values against the unfused head's: by the mean value theorem they differ by the maps' differences
+    times the decode's slopes (2 s stride / 4 of a centre, 32/27 anchor of a size, 1/4 of a score), and by the decode's own roundings, eight
+    half steps of each."""
+    from object_detection_amd.layers import head_convs
+    from object_detection_amd.yolo import Detect
+    dtype = torch.float16 if half else torch.float32
+    torch.manual_seed(4)
+    strides = torch.tensor([8.0, 16.0, 32.0])
+    det = Detect(20, [[10, 13, 16, 30, 33, 23], [30, 61, 62, 45, 59, 119], [116, 90, 156, 198, 373, 326]], (16, 32, 64)).cuda()
+    det.stride = strides
+    det.anchors /= strides.view(-1, 1, 1).cuda()
+    det = det.to(dtype).eval()
+    det.lazy_maps = lazy
+    feats = [torch.randn(3, c, s, s + 2, device="cuda").to(dtype) for c, s in ((16, 24), (32, 12), (64, 6))]
+    with torch.no_grad():
+        det.fused_convs = False
+        z0, maps0 = det(list(feats))
+        det.fused_convs = True
+        z1, maps1 = det(list(feats))
+        rows = det.detections(list(feats), 0.3, 0.5)
+        convs = head_convs(feats, [m.weight for m in det.m], [m.bias for m in det.m])
+        for f, m, y in zip(feats, det.m, convs):
+            close(to_rows(y), rows64(to_rows(f).detach(), m.weight.detach().flatten(1), m.bias.detach(), None, None)["y"], "convolution")
+        own = list(det.m)
+        det.m = torch.nn.ModuleList([_Given(m, y) for m, y in zip(own, convs)])
+        z2, maps2 = det(list(feats))
+        given = det.detections(list(feats), 0.3, 0.5)
+    assert torch.equal(z1, z2) and z1.dtype == z0.dtype and z1.shape == z0.shape
+    assert len(maps1) == 3 and all(torch.equal(a, b) for a, b in zip(maps1, maps2))
+    assert len(rows) == len(given) == 3 and sum(len(r) for r in rows) > 20
+    assert all(torch.equal(a, b) for a, b in zip(rows, given))
+    slopes, apart = [], []
+    for l, (a, b) in enumerate(zip(maps0, maps1)):
+        slope = torch.full((3, 25), 0.25, dtype=torch.float64, device="cuda")
+        slope[:, :2] = 0.5 * float(strides[l])
+        slope[:, 2:4] = 32 / 27 * (det.anchors[l].double() * float(strides[l]))
+        slopes.append((slope[None, :, None, None, :] * (a.double() - b.double()).abs()).reshape(3, -1, 25))
+        apart.append(torch.full_like(slopes[-1], float(strides[l])))
+    bound = torch.cat(slopes, 1) + 8 * torch.finfo(dtype).eps / 2 * (torch.cat(apart, 1) + z0.double().abs()) * 2
+    assert bool(((z0.double() - z1.double()).abs() <= bound).all())
+    assert bool(torch.cat(slopes, 1).max() < 1.0)                       # (the bound says something)
