@@ -1,8 +1,9 @@
 """The norm of all gradients of a training step taken as one vector, and clipping by it.
 
-What stands between ComputeLoss / the layers' gradients and the optimizer in a step of object_detection/yolov5/train.py:337-346
-(scaler.scale(loss).backward(); scaler.step(optimizer)): the gradients carry a loss scale there, which both calls can take out on
-the way.  Two launches for up to 280 tensors of one type (176 with other tensors for the results), no host synchronisation, sums
+What stands between ComputeLoss / the layers' gradients and the optimizer in a step of object_detection/yolov5/train.py:337-346:
+scaler.scale(loss).backward(); scaler.unscale_(optimizer); clip_grad_norm_(...); scaler.step(optimizer).  A GradScaler takes its scale
+out itself (in step(), if unscale_() has not), so `scale` stays away from it; `scale` is for loops that multiply the loss, divide by the
+scale and skip overflowed steps on their own.  Two launches for up to 280 tensors of one type (176 with other tensors for the results), no host synchronisation, sums
 in double, results repeat bit for bit.
 """
 import torch

@@ -450,3 +450,37 @@ def test_strided_gradients_that_share_memory_are_refused():
     # read as often as one likes: an expanded gradient counts each of its elements, into other tensors
     n, out = clip_grads([row.expand(4, 8), wide[:, 2:5], wide[:, 2:5]], 1e9)
     near(n, norm64([row.expand(4, 8), wide[:, 2:5], wide[:, 2:5]], 2.0))
+
+
+def test_the_documented_order_with_a_grad_scaler():
+    """scale, backward, unscale_, clip_grad_norm_, step: the weights of a step without a scaler whose gradients were clipped by the formula;
+    an overflowed step changes nothing.  And `scale` in a loop of its own: the same weights."""
+    from object_detection_amd.grads import clip_grad_norm_, clip_grads
+    g = made([(40, 16), (40,)], torch.float32, 30)
+    start = [torch.zeros_like(v) for v in g]
+    norm = norm64(g, 2.0)
+
+    def loss_of(ps):
+        return sum((p * v).sum() for p, v in zip(ps, g))          # its gradients are g
+    ps = [torch.nn.Parameter(s.clone()) for s in start]
+    optimizer = torch.optim.SGD(ps, lr=1.0)
+    scaler = torch.amp.GradScaler("cuda", init_scale=1024.0)
+    scaler.scale(loss_of(ps)).backward()
+    scaler.unscale_(optimizer)
+    near(clip_grad_norm_(ps, norm / 4), norm)
+    scaler.step(optimizer)
+    scaler.update()
+    clipped_close([-p for p in ps], g, norm, norm / 4)
+    after = [p.detach().clone() for p in ps]
+    optimizer.zero_grad()
+    scaler.scale(loss_of(ps) * float("inf")).backward()
+    scaler.unscale_(optimizer)
+    assert not math.isfinite(float(clip_grad_norm_(ps, norm / 4)))
+    scaler.step(optimizer)
+    scaler.update()
+    assert all(torch.equal(p, a) for p, a in zip(ps, after)) and scaler.get_scale() == 512.0
+    own = [torch.nn.Parameter(s.clone()) for s in start]
+    (loss_of(own) * 1024.0).backward()
+    n = clip_grad_norm_(own, norm / 4, scale=1024.0)
+    near(n, norm)
+    clipped_close([p.grad for p in own], g, norm, norm / 4)
