@@ -8,6 +8,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 
 #include "../../include/dethead.h"
@@ -73,11 +74,15 @@ struct Item {
 // The kernels read memory: a view whose sign is kept beside it (the imaginary part of a conjugate) is written out first.
 Tensor in_memory(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 
-// Kernels carry no tangents: a dual tensor is refused, its derivative not taken for zero.
+// Kernels carry no tangents: a dual tensor is refused, its derivative not taken for zero.  Asked of the tensors only where a level of
+// forward mode is open (a view's answer costs 15 ns).
+bool dual_level()
+{
+    return c10::AutogradState::get_tls_state().get_fw_grad_mode() && torch::autograd::ForwardADLevel::try_get_by_idx(0);
+}
 void refuse_dual(const char* where, const Tensor& t)
 {
-    if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
-        fail(std::string(where) + ": forward-mode derivatives are not offered");
+    if (t._fw_grad(0).defined()) fail(std::string(where) + ": forward-mode derivatives are not offered");
 }
 
 // One supported type on one ROCm device; under autocast its type.
@@ -87,8 +92,9 @@ void check_tensors(const char* where, Item& it)
         fail(std::string(where) + ": x is on " + it.x.device().str() + ": object_detection_amd only runs on ROCm devices (no CPU fallback)");
     for (Tensor* t : it.all())
         if (t->defined() && t->is_neg()) *t = t->resolve_neg();
-    for (Tensor* t : it.all())
-        if (t->defined()) refuse_dual(where, *t);
+    if (dual_level())
+        for (Tensor* t : it.all())
+            if (t->defined()) refuse_dual(where, *t);
     for (Tensor* t : it.all())
         if (t->defined() && t->device() != it.x.device())
             fail(std::string(where) + ": tensors on " + t->device().str() + " and " + it.x.device().str());
@@ -461,12 +467,13 @@ bool dense(const Tensor& t) { return t.is_contiguous() || t.is_non_overlapping_a
 std::vector<List> listed(const char* where, const variable_list& grads, variable_list* read)
 {
     std::vector<List> lists;
+    const bool dual = dual_level();
     for (size_t k = 0; k < grads.size(); ++k) {
         const Tensor& g = grads[k];
         if (!g.is_cuda())
             fail(std::string(where) + ": a gradient is on " + g.device().str() + ": object_detection_amd only runs on ROCm devices (no CPU fallback)");
         if (g.layout() != at::kStrided) fail(std::string(where) + ": gradients must be dense tensors");
-        refuse_dual(where, g);
+        if (dual) refuse_dual(where, g);
         if (g.device() != grads[0].device()) fail(std::string(where) + ": gradients on " + grads[0].device().str() + " and " + g.device().str());
         const at::ScalarType type = g.scalar_type();
         if (code_of(type) < 0) fail(std::string(where) + ": gradients must be fp32, fp16 or bf16, got " + c10::toString(type));

@@ -855,3 +855,15 @@ def test_a_fused_head_in_eval(lazy, half):
     bound = torch.cat(slopes, 1) + 8 * torch.finfo(dtype).eps / 2 * (torch.cat(apart, 1) + z0.double().abs()) * 2
     assert bool(((z0.double() - z1.double()).abs() <= bound).all())
     assert bool(torch.cat(slopes, 1).max() < 1.0)                       # (the bound says something)
+
+
+def test_function_transforms_are_refused():
+    """torch.func's wrapped tensors have no memory of their own: an error, not a result without the transform."""
+    from object_detection_amd.grads import total_grad_norm
+    from object_detection_amd.layers import linear
+    x, w = made((3, 5, 8), torch.float32, 1).cuda(), made((6, 8), torch.float32, 2).cuda()
+    for call in (lambda: torch.func.jvp(lambda v: linear(v, w), (x,), (torch.ones_like(x),)), lambda: torch.func.vmap(lambda v: linear(v, w))(x),
+                 lambda: torch.func.grad(lambda v: linear(v, w).sum())(x), lambda: torch.func.vmap(lambda v: total_grad_norm([v]))(x),
+                 lambda: torch.func.jvp(lambda v: total_grad_norm([v]), (x,), (torch.ones_like(x),))):
+        with pytest.raises(RuntimeError):
+            call()
