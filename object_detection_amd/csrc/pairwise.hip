@@ -14,8 +14,8 @@
 // Tiles are numbered column-first in a one-dimensional grid (no 65 535 limit on either side).  When M is not a multiple
 // of four, or a pointer is not 16-byte aligned, one column per lane and 4-byte accesses.  The quotient is the IEEE
 // division the reference performs, bit for bit: either the division itself or, for tiles whose boxes are all "plain", the
-// same refinement sequence without its range handling and on two pairs per instruction (pw_div2_plain; 47 -> 44 us at
-// 8192 x 8192, 6.0 TB/s, against 42 us for the same stores with no arithmetic at all).
+// same refinement sequence without its range handling (pw_div2_plain; 47 -> 44 us at 8192 x 8192, 6.1 TB/s, against 42 us for
+// the same stores with no arithmetic at all).
 #include "dh_common.h"
 #include "../../include/dethead.h"
 
@@ -38,12 +38,11 @@ __device__ __forceinline__ float pw_iou(const float4 r, float ra, float cx, floa
 
 typedef float dh_f2 __attribute__((ext_vector_type(2)));
 
-// n / d of two pairs at once, correctly rounded for operands in the "plain" range (below).  The instruction sequence is the
+// n / d of two pairs, correctly rounded for operands in the "plain" range (below).  The instruction sequence is the
 // one the compiler expands an IEEE fp32 division into -- reciprocal estimate, one refinement of it, two refinements of the
 // quotient -- without the three instructions around it that only matter outside that range (v_div_scale of numerator and
-// denominator, v_div_fixup): 7 vector instructions per quotient instead of 10.  The kernel is bound by exactly those
-// instructions at write-bound sizes (counters with the full division: 24 per element, the vector ALU busy for 41 of 47 us at
-// 8192 x 8192).
+// denominator, v_div_fixup): 8 vector instructions per quotient, the quarter-rate reciprocal among them, instead of 11.  26 per
+// element in all at 8192 x 8192, waves waiting for the vector ALU 46 % of their time: it and the stores bound the kernel together.
 __device__ __forceinline__ dh_f2 pw_div2_plain(const dh_f2 n, const dh_f2 d)
 {
     const dh_f2 one = {1.0f, 1.0f};
