@@ -1203,6 +1203,10 @@ int launch(const Launch& L, bool arc, bool brc, bool aligned, const Shape& t, hi
 // dy is [outer][n][inner]; the bias gradient sums over outer and inner.  One pass over dy and z in 16-byte pieces (of any
 // alignment): a wave takes rows of `inner` values of one n (maps), or the same 64 pieces of columns in every row (inner = 1).
 // Sums go to the workspace, SPLIT of them at most per n, and are added in order by k_bias_join.
+// Two roundings to 16 bits are choices: z is kept in the tensors' type between forward and backward (in fp32 it would be half of what a
+// forward pass with an activation writes and the slope reads again), and dz is rounded to it because the matrix instructions that
+// read it take 16 bits; the bias gradient sums it before that.  Gradients are then off by two half steps instead of one: 8192 x 1024 ->
+// 1024 bf16 0.0024 from 64 bits, 0.0017 with both in fp32.
 constexpr int BIAS_SPLIT = 256;
 
 // v[k] = dy * act'(z), stored where dz is; the values count from `at` in one piece of V, `n` of them exist
