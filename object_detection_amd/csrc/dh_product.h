@@ -59,7 +59,6 @@ template <bool FAST> struct Act<DH_ACT_NONE, FAST> {
 };
 template <bool FAST> struct Act<DH_ACT_RELU, FAST> {
     __device__ static float value(float z) { return z > 0.f ? z : (z != z ? z : 0.f); }      // a NaN stays one
-    __device__ static float slope(float z) { return z > 0.f ? 1.f : 0.f; }
 };
 template <bool FAST> __device__ __forceinline__ float logistic(float z)
 {
@@ -95,6 +94,13 @@ template <bool FAST> struct Act<DH_ACT_GELU, FAST> {
     __device__ static float value(float z) { float bell; return z * normal(z, &bell); }
     __device__ static float slope(float z) { float bell; const float n = normal(z, &bell); return fmaf(z * 0.39894228040143268f, bell, n); }
 };
+
+// dy act'(z).  A relu passes dy on or stops it: an infinite dy where it stops is 0, and a NaN z passes, as in torch.
+template <int ACT, bool FAST> __device__ __forceinline__ float act_back(float dy, float z)
+{
+    if constexpr (ACT == DH_ACT_RELU) return z <= 0.f ? 0.f : dy;
+    else return dy * Act<ACT, FAST>::slope(z);
+}
 
 // f.template operator()<ACT>() for the activation of a launch
 template <typename F> __device__ __forceinline__ void with_act(int act, F&& f)
@@ -1230,7 +1236,7 @@ __device__ __forceinline__ void slope_piece(const T* dy, const T* z, T* dz, int6
     if (!z) return;
     with_act(act, [&](auto a) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] *= Act<decltype(a)::value, sizeof(T) == 2>::slope(Elem<T>::up(y[k]));
+        for (int k = 0; k < V; ++k) v[k] = act_back<decltype(a)::value, sizeof(T) == 2>(v[k], Elem<T>::up(y[k]));
     });
 #pragma unroll
     for (int k = 0; k < V; ++k) g[k] = Elem<T>::down(v[k]);
@@ -1269,7 +1275,7 @@ __device__ __forceinline__ void slope_pieces(const T* dy, const T* z, T* dz, int
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[u][k] *= Act<decltype(a)::value, sizeof(T) == 2>::slope(Elem<T>::up(y[u][k]));
+            for (int k = 0; k < V; ++k) v[u][k] = act_back<decltype(a)::value, sizeof(T) == 2>(v[u][k], Elem<T>::up(y[u][k]));
     });
 #pragma unroll
     for (int u = 0; u < U; ++u) {

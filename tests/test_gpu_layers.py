@@ -867,3 +867,26 @@ def test_function_transforms_are_refused():
                  lambda: torch.func.jvp(lambda v: total_grad_norm([v]), (x,), (torch.ones_like(x),))):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [True, False])
+def test_a_relu_stops_what_it_stops(rows, dtype):
+    """The gradient of a relu is dy or 0: infinities and NaN in dy go no further where z is not positive, and reach x where it is; a NaN
+    in z lets dy through.  As torch's relu, value by value."""
+    from object_detection_amd.layers import linear, pointwise_conv
+    inf, nan = float("inf"), float("nan")
+    z, dy = torch.meshgrid(torch.tensor([-inf, -2.0, -0.0, 0.0, 1e-6, 3.0, inf, nan]), torch.tensor([1.0, -2.0, 0.0, inf, -inf, nan]), indexing="ij")
+    z, dy = z.reshape(-1).to(dtype), dy.reshape(-1).to(dtype)
+    n = z.numel()
+    x = (z[:, None] if rows else z.view(1, 1, 6, 8)).cuda().requires_grad_(True)
+    g = (dy[:, None] if rows else dy.view(1, 1, 6, 8)).cuda()
+    one, bias = torch.ones(1, 1, dtype=dtype, device="cuda"), torch.zeros(1, dtype=dtype, device="cuda", requires_grad=True)
+    y = (linear if rows else pointwise_conv)(x, one, bias, "relu")
+    y.backward(g)
+    ref = x.detach().clone().requires_grad_(True)
+    want = torch.relu(ref)
+    want.backward(g)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.nan_to_num(y), torch.nan_to_num(want))
+    assert torch.equal(torch.isnan(x.grad), torch.isnan(ref.grad)) and torch.equal(torch.nan_to_num(x.grad), torch.nan_to_num(ref.grad))
+    assert torch.isnan(bias.grad).all()
