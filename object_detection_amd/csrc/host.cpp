@@ -516,6 +516,7 @@ Tensor scale_on(const char* where, const py::object& scale, const Tensor& like)
     if (THPVariable_Check(scale.ptr())) {
         const Tensor t = scale.cast<Tensor>();
         if (t.numel() != 1) fail(std::string(where) + ": scale must be one number, got shape " + shape(t));
+        if (t.is_cpu()) return at::full({}, t.detach().item<double>(), like.options().dtype(at::kFloat));      // no copy to wait for
         return t.detach().to(like.device(), at::kFloat);
     }
     const double v = scale.cast<double>();

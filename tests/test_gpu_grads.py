@@ -484,3 +484,23 @@ def test_the_documented_order_with_a_grad_scaler():
     n = clip_grad_norm_(own, norm / 4, scale=1024.0)
     near(n, norm)
     clipped_close([p.grad for p in own], g, norm, norm / 4)
+
+
+def test_a_scale_on_the_host_can_be_captured():
+    """A one-element tensor in host memory is a number: nothing is copied, so the call can be captured."""
+    from object_detection_amd.grads import clip_grads, total_grad_norm
+    grads = made([(100,), (9000,)], torch.float32, 40)
+    scale = torch.tensor([8.0], dtype=torch.float64)
+    out = [torch.empty_like(g) for g in grads]
+    norm = norm64(grads, 2.0, 8.0)
+    near(total_grad_norm(grads, scale=scale), norm)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        n, _ = clip_grads(grads, norm / 2, scale=scale, out=out)
+    for _ in range(3):
+        for o in out:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        near(n, norm)
+        clipped_close(out, grads, norm, norm / 2, 8.0)
