@@ -559,7 +559,7 @@ __device__ __forceinline__ void epilogue(f4 (&acc)[TI][TJ], const Plan& q, int a
 // Aligned operands: a ring of STAGES buffers in LDS, the copies of STAGES - 1 steps on their way while one is multiplied (copied by
 // the memory system itself, so that a step costs no registers and one barrier).
 // Large reductions are bound by the matrix pipes: 8192^3 bf16 1357 TFLOP/s; with 1024 to reduce the prologue and the epilogue of
-// a tile show, 8192 x 1024 -> 4096 bf16 69 us = 999 TFLOP/s, with gelu 80 (862).  Maps with few channels are bound by bytes: 128 ->
+// a tile show, 8192 x 1024 -> 4096 bf16 71 us = 968 TFLOP/s, with gelu 81 (848).  Maps with few channels are bound by bytes: 128 ->
 // 128 channels, silu and residual of 64 x 80 x 80 cells (315 MB) 75 us = 4.2 TB/s, where a plain copy of that card reaches 4.9.
 template <typename T, int BI, int BJ, int BR, int WI, int WJ, int STAGES, int WAVES, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64, WAVES) k_product(const Launch L)
@@ -802,10 +802,6 @@ __device__ __forceinline__ Split split(u4 v, uint32_t* smallest)
     return s;
 }
 
-// fp32 products, six bf16 ones each (above).  Long reductions are bound by the vector instructions that split beside the matrix
-// instructions that multiply: 8192 x 1024 -> 4096 357 us = 193 TFLOP/s, 8192^3 195, where the card's fp32 matrix instructions end at
-// 157.  The head's levels at batch 64 (548 MB of 915 written) take 400 us: 266 of memory and 283 of products, which overlap between
-// the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
 // The largest magnitude in a wave's values (a NaN is passed over: its sums are done again anyway).
 template <int N> __device__ __forceinline__ void most_of(const u4* v, float* most)
 {
@@ -821,6 +817,10 @@ __device__ __forceinline__ float wave_most(float v)
     return v;
 }
 
+// fp32 products, six bf16 ones each (above).  Long reductions are bound by the vector instructions that split beside the matrix
+// instructions that multiply: 8192 x 1024 -> 4096 366 us = 188 TFLOP/s, 8192^3 198, where the card's fp32 matrix instructions end at
+// 157.  The head's levels at batch 64 (548 MB of 915 written) take 404 us: 266 of memory and 283 of products, which overlap between
+// the two workgroups of a CU only in part.  Few tiles (1023 x 777 -> 1001, 23 us) wait for their steps one by one.
 template <int BI, int BJ, int WI, int WJ, int DEPTH, int WAVES, int GROUPS, bool ARC, bool BRC>
 __global__ void __launch_bounds__(WI * WJ * 64 * GROUPS, WAVES) k_product_split(const Launch L)
 {
