@@ -557,7 +557,8 @@ int dh_products(const dh_product* products, int n, int dtype, int activation, vo
 
 /* The two other steps of those products' backward pass, in one read of dy: dz = dy * act'(z) (skipped when z is null) and the
  * bias gradient dbias[c] = sum over outer and inner of dz (skipped when dbias is null; summed before dz is rounded).  dy, z
- * and dz are contiguous [outer][n][inner]: maps have inner = cells, rows inner = 1.  workspace: device,
+ * and dz are contiguous [outer][n][inner]: maps have inner = cells, rows inner = 1; without elements (outer or inner 0) dbias is zero
+ * and nothing else is touched.  A relu passes dy where z is not <= 0 and stops it elsewhere.  workspace: device,
  * dh_product_slope_workspace(n) bytes when dbias is given. */
 size_t dh_product_slope_workspace(int64_t n);
 int dh_product_slope(const void* dy, const void* z, void* dz, void* dbias, int64_t outer, int64_t n, int64_t inner,
